@@ -1,4 +1,4 @@
-"""ctypes binding of libbof_hip.so (the C ABI declared in include/bof_hip.h).
+"""ctypes binding of libbof_hip.so (the C ABI declared in include/bof_hip.h and include/bof_f8.h).
 
 Used by tests/, bench.py and __graft_entry__.py.  Device memory is passed as raw
 pointers (e.g. torch.Tensor.data_ptr()); streams as hipStream_t handles
@@ -129,6 +129,19 @@ SYMBOLS = [
     ("bof_gen_sparse_rows", C.c_int, [i64, i64, i64, i64, P, P, P, P]),
 ]
 
+# every symbol include/bof_f8.h declares
+SYMBOLS_F8 = [
+    ("bof_f8_gemm", C.c_int, [i64, i64, i64, f32, P, i64, C.c_int, P, i64, C.c_int, P, i64, C.c_int, P, i64, C.c_int, f32, P, i64,
+                              C.c_int, P, u64, P]),
+    ("bof_f8_gemm_workspace_bytes", u64, [i64, i64, i64]),
+    ("bof_f8_quant", C.c_int, [i64, i64, P, i64, C.c_int, C.c_int, C.c_int, P, i64, P, i64, P, i64, P, i64, P]),
+    ("bof_rmsnorm_f8", C.c_int, [i64, i64, C.c_int, P, i64, P, i64, P, f32, P, i64, C.c_int, P, i64, P, i64, P, i64, P, P]),
+    ("bof_rmsnorm_grad", C.c_int, [i64, i64, C.c_int, P, i64, P, i64, P, P, P, i64, P, i64, f32, P, P, u64, P]),
+    ("bof_rmsnorm_grad_workspace_bytes", u64, [i64, i64]),
+]
+# element types of bof_f8.h
+F32, BF16, F16, E4M3, E5M2 = range(5)
+
 
 def build(verbose=False):
     """Compile libbof_hip.so for gfx950 in-tree (hipcc cross-compiles without a GPU)."""
@@ -154,7 +167,7 @@ def lib():
             raise BofError(f"{LIB_PATH} is missing: run `make -C {HERE}` "
                            "(or __graft_entry__.build()); there is no CPU fallback")
         L = C.CDLL(LIB_PATH)
-        for name, res, args in SYMBOLS:
+        for name, res, args in SYMBOLS + SYMBOLS_F8:
             fn = getattr(L, name)  # AttributeError if the .so does not export it
             fn.restype = res
             fn.argtypes = args
@@ -218,6 +231,45 @@ def scsrgemv(trans, m, n, val, ptr, col, x, y, stream=0):
 
 def scsrcsc(m, n, nnz, val, ptr, col, val_tr, ptr_tr, col_tr, stream=0):
     check(lib().bof_scsrcsc(m, n, nnz, val, ptr, col, val_tr, ptr_tr, col_tr, stream), "bof_scsrcsc")
+
+
+# ---- 8-bit floating point (include/bof_f8.h) ---------------------------------------
+def f8_gemm(m, n, k, alpha, a, lda, a_type, sa, ldsa, ga, b, ldb, b_type, sb, ldsb, gb, beta, c, ldc, c_type, work=0,
+            work_bytes=0, stream=0):
+    """C (m x n) = alpha * A * B^T + beta * C; A (m x k) and B (n x k) in 8 bits with a scale for each ga (gb) x 128 block."""
+    rc = lib().bof_f8_gemm(m, n, k, alpha, a, lda, a_type, sa, ldsa, ga, b, ldb, b_type, sb, ldsb, gb, beta, c, ldc, c_type, work,
+                           work_bytes, stream)
+    if rc:
+        check(rc, "bof_f8_gemm")
+
+
+def f8_gemm_workspace_bytes(m, n, k):
+    return lib().bof_f8_gemm_workspace_bytes(m, n, k)
+
+
+def f8_quant(rows, cols, x, ldx, x_type, f8_type, group, q, ldq, s, lds, qt=0, ldqt=0, st=0, ldst=0, stream=0):
+    """X (rows x cols) in 8 bits: as it lies (q, s), transposed (qt, st), or both; 0 for what is not wanted."""
+    rc = lib().bof_f8_quant(rows, cols, x, ldx, x_type, f8_type, group, q, ldq, s, lds, qt, ldqt, st, ldst, stream)
+    if rc:
+        check(rc, "bof_f8_quant")
+
+
+def rmsnorm_f8(rows, n, type_, x, ldx, r, ldr, w, eps, h, ldh, f8_type, q, ldq, s, lds, y=0, ldy=0, rstd=0, stream=0):
+    """h = x + r, the norm of its rows times w in 8 bits (q, s) and in `type_` (y), and rstd; 0 for what is not wanted."""
+    rc = lib().bof_rmsnorm_f8(rows, n, type_, x, ldx, r, ldr, w, eps, h, ldh, f8_type, q, ldq, s, lds, y, ldy, rstd, stream)
+    if rc:
+        check(rc, "bof_rmsnorm_f8")
+
+
+def rmsnorm_grad(rows, n, type_, dy, lddy, h, ldh, w, rstd, dh, lddh, dx, lddx, beta=0.0, dw=0, work=0, work_bytes=0, stream=0):
+    """dx and dw = beta * dw + ... of the norm; dh: the gradient that reaches h past the norm, or 0; dw 0: not wanted."""
+    rc = lib().bof_rmsnorm_grad(rows, n, type_, dy, lddy, h, ldh, w, rstd, dh, lddh, dx, lddx, beta, dw, work, work_bytes, stream)
+    if rc:
+        check(rc, "bof_rmsnorm_grad")
+
+
+def rmsnorm_grad_workspace_bytes(rows, n):
+    return lib().bof_rmsnorm_grad_workspace_bytes(rows, n)
 
 
 # ---- planning ----------------------------------------------------------------------
