@@ -27,6 +27,90 @@ __device__ __forceinline__ void store_dense(void *p, int64_t i, float v) {
   else if constexpr (T == BOF_BF16) ((__bf16 *) p)[i] = (__bf16) v;
   else ((_Float16 *) p)[i] = (_Float16) v;
 }
+// Eight neighbours as they lie in memory.  Any alignment of the element type: the loads and stores are 16 bytes wide whatever
+// the address (gfx950 takes them unaligned).  `valid` elements exist (any number; the others read as 0 and are not written).
+template <int T>
+struct Eight {
+  u32x4 w[T == BOF_F32 ? 2 : 1];
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (T == BOF_F32) return __uint_as_float(w[e >> 2][e & 3]);
+    const uint32_t u = w[0][e >> 1];
+    if constexpr (T == BOF_BF16) return __uint_as_float(e & 1 ? u & 0xffff0000u : u << 16);
+    const uint16_t b = (uint16_t) (e & 1 ? u >> 16 : u);
+    return (float) __builtin_bit_cast(_Float16, b);
+  }
+};
+template <int T>
+__device__ __forceinline__ Eight<T> load_eight(const void *p, int64_t i, int64_t valid) {
+  Eight<T> r;
+  constexpr int z = T == BOF_F32 ? 4 : 2;
+  const uint8_t *from = (const uint8_t *) p + i * z;
+  if (valid >= 8) {
+    __builtin_memcpy(&r, from, 8 * z);
+  } else {
+    r.w[0] = u32x4{0u, 0u, 0u, 0u};
+    if constexpr (T == BOF_F32) r.w[1] = r.w[0];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < valid) {
+        if constexpr (T == BOF_F32) r.w[e >> 2][e & 3] = ((const uint32_t *) from)[e];
+        else r.w[0][e >> 1] |= (uint32_t) ((const uint16_t *) from)[e] << (16 * (e & 1));
+      }
+  }
+  return r;
+}
+template <int T>
+__device__ __forceinline__ void store_eight(void *p, int64_t i, const float (&v)[8], int64_t valid) {
+  if (valid >= 8) {
+    if constexpr (T == BOF_F32) {
+      __builtin_memcpy((float *) p + i, v, 32);
+    } else if constexpr (T == BOF_BF16) {
+      __bf16 o[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = (__bf16) v[e];
+      __builtin_memcpy((__bf16 *) p + i, o, 16);
+    } else {
+      _Float16 o[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) o[e] = (_Float16) v[e];
+      __builtin_memcpy((_Float16 *) p + i, o, 16);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < valid) store_dense<T>(p, i + e, v[e]);
+  }
+}
+// eight bytes, of which `valid` are written
+__device__ __forceinline__ void store_bytes(uint8_t *p, uint64_t v, int64_t valid) {
+  if (valid >= 8) {
+    __builtin_memcpy(p, &v, 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < valid) p[e] = (uint8_t) (v >> (8 * e));
+  }
+}
+
+// ---- reductions over lanes ----------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ uint32_t lanes(uint32_t v) { return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, 0xf, 0xf, true); }
+// over each 16 neighbouring lanes, for all of them: lane ^ 1, lane ^ 2, then the mirrors of 8 and of 16
+__device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
+  m = max(m, lanes<0xB1>(m));
+  m = max(m, lanes<0x4E>(m));
+  m = max(m, lanes<0x141>(m));
+  return max(m, lanes<0x140>(m));
+}
+__device__ __forceinline__ float sum_of_wave(float v) {
+  v += __uint_as_float(lanes<0xB1>(__float_as_uint(v)));
+  v += __uint_as_float(lanes<0x4E>(__float_as_uint(v)));
+  v += __uint_as_float(lanes<0x141>(__float_as_uint(v)));
+  v += __uint_as_float(lanes<0x140>(__float_as_uint(v)));
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
 constexpr int dense_bytes(int type) { return type == BOF_F32 ? 4 : 2; }
 
 // ---- 8-bit elements and their scales ------------------------------------------------
@@ -41,22 +125,22 @@ __device__ __forceinline__ uint32_t finite_magnitude(float v) {
 // E8M0 code of the smallest power of two, at least 2^-126, that brings a magnitude (its bits) into the type's range.
 // amax = 1.f * 2^(E-127) = (1.f / 2) * 2^(E-126) fits 0.875 * 2^(TOP + e) from e = E - 126 - TOP on, one more where
 // 1.f > 1.75.  The codes lie in [1, 247]: a scale and its reciprocal are both normal floats.
-template <int F8>
-__device__ __forceinline__ uint32_t scale_code(uint32_t amax_bits) {
-  const int c = (int) (amax_bits >> 23) + 1 - f8_top(F8) + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+__device__ __forceinline__ uint32_t scale_code(uint32_t amax_bits, int top) {
+  const int c = (int) (amax_bits >> 23) + 1 - top + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return amax_bits == 0 ? 127u : (uint32_t) max(c, 1);
 }
 __device__ __forceinline__ float scale_inverse(uint32_t code) { return __uint_as_float((254u - code) << 23); }
-// two floats, already divided by their scale, to two bytes (nearest even; a NaN stays NaN, an infinity becomes the
-// type's NaN or infinity: the conversion instructions do that)
-template <int F8, bool HI>
-__device__ __forceinline__ uint32_t f8_pair(float a, float b, uint32_t old) {
-  if constexpr (F8 == BOF_E4M3) return (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(a, b, (int) old, HI);
-  return (uint32_t) __builtin_amdgcn_cvt_pk_bf8_f32(a, b, (int) old, HI);
-}
-template <int F8>
-__device__ __forceinline__ uint32_t f8_quad(float a, float b, float c, float d) {
-  return f8_pair<F8, true>(c, d, f8_pair<F8, false>(a, b, 0u));
+// eight floats times inv to eight bytes (nearest even; a NaN stays NaN, an infinity becomes the type's NaN or infinity:
+// the conversion instructions do that).  top = f8_top(type) names the type.
+__device__ __forceinline__ uint64_t f8_eight(const float (&v)[8], float inv, int top) {
+  uint32_t o[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const float a = v[4 * h] * inv, b = v[4 * h + 1] * inv, c = v[4 * h + 2] * inv, d = v[4 * h + 3] * inv;
+    if (top == 9) o[h] = (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+    else o[h] = (uint32_t) __builtin_amdgcn_cvt_pk_bf8_f32(c, d, __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false), true);
+  }
+  return o[0] | (uint64_t) o[1] << 32;
 }
 
 // ---- entry points -------------------------------------------------------------------

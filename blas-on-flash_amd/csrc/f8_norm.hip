@@ -12,123 +12,221 @@ struct Quant {
   int64_t ldx, rows, cols;
   uint8_t *q, *s, *qt, *st;
   int64_t ldq, lds, ldqt, ldst;
+  int top;
 };
 
-// One workgroup, one 128 x 128 block of X through LDS.  A thread pair owns a row (64 elements each), and in the second
-// half a column.
-template <int X, int F8, int GROUP>
-__global__ void __launch_bounds__(256) quant_tile_kernel(Quant p) {
-  __shared__ float tile[128][129];
-  __shared__ uint32_t top[256];
-  const int t = threadIdx.x;
-  const int64_t tiles_c = (p.cols + 127) >> 7;
-  const int64_t bi = blockIdx.x / tiles_c, bj = blockIdx.x % tiles_c;
+// One workgroup, one 128 x 128 block of X, which is read once and stays in registers: thread t holds an 8 x 8 block, columns
+// 8 * (t & 15), rows 8 * (t >> 4).  The largest magnitude of a row of the block is then that of 16 neighbouring lanes, that
+// of a column is joined through LDS.  Transposed elements pass through LDS: a thread's eight rows of a column are eight
+// neighbouring bytes there, a unit; column c keeps its 16 units XOR-ed with c / 8, so that neither the writes (16 lanes,
+// 16 columns) nor the reads meet a bank twice.
+template <int X, int GROUP, bool T>
+__global__ void __launch_bounds__(256) quant_kernel(Quant p) {
+  __shared__ uint64_t turned[T ? 128 * 16 : 1];
+  __shared__ uint32_t top[4][128];
+  const int t = threadIdx.x, c8 = (t & 15) * 8, r8 = (t >> 4) * 8;
+  const int64_t tiles_c = (p.cols + 127) >> 7, bi = blockIdx.x / tiles_c, bj = blockIdx.x % tiles_c;
   const int64_t r0 = bi * 128, c0 = bj * 128;
   const int nr = (int) min((int64_t) 128, p.rows - r0), nc = (int) min((int64_t) 128, p.cols - c0);
-  for (int at = t; at < 128 * 128; at += 256) {
-    const int r = at >> 7, c = at & 127;
-    tile[r][c] = r < nr && c < nc ? load_dense<X>(p.x, (r0 + r) * p.ldx + c0 + c) : 0.f;
+  Eight<X> x[8];
+#pragma unroll
+  for (int u = 0; u < 8; u++) x[u] = load_eight<X>(p.x, (r0 + r8 + u) * p.ldx + c0 + c8, r8 + u < nr ? nc - c8 : 0);
+  uint32_t row_top[8], col_top[8] = {};
+#pragma unroll
+  for (int u = 0; u < 8; u++) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const uint32_t v = finite_magnitude(x[u].at(e));
+      m = max(m, v);
+      if (T && GROUP == 1) col_top[e] = max(col_top[e], v);
+    }
+    row_top[u] = max_of_16(m);
+  }
+  if (GROUP == 128) {   // one scale for all of it
+    uint32_t m = row_top[0];
+#pragma unroll
+    for (int u = 1; u < 8; u++) m = max(m, row_top[u]);
+    m = max(m, (uint32_t) __shfl_xor((int) m, 16));
+    m = max(m, (uint32_t) __shfl_xor((int) m, 32));
+    if ((t & 63) == 0) top[t >> 6][0] = m;
+    __syncthreads();
+    m = max(max(top[0][0], top[1][0]), max(top[2][0], top[3][0]));
+#pragma unroll
+    for (int u = 0; u < 8; u++) { row_top[u] = m; col_top[u] = m; }
+  } else if (T) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      col_top[e] = max(col_top[e], (uint32_t) __shfl_xor((int) col_top[e], 16));
+      col_top[e] = max(col_top[e], (uint32_t) __shfl_xor((int) col_top[e], 32));
+    }
+    if ((t & 48) == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) top[t >> 6][c8 + e] = col_top[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; e++) col_top[e] = max(max(top[0][c8 + e], top[1][c8 + e]), max(top[2][c8 + e], top[3][c8 + e]));
+  }
+  if (!T || p.q) {
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const uint32_t code = scale_code(row_top[u], p.top);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = x[u].at(e);
+      if (r8 + u < nr) {
+        store_bytes(p.q + (r0 + r8 + u) * p.ldq + c0 + c8, f8_eight(v, scale_inverse(code), p.top), nc - c8);
+        if ((t & 15) == 0 && (GROUP == 1 || r8 + u == 0)) p.s[(GROUP == 1 ? r0 + r8 + u : bi) * p.lds + bj] = (uint8_t) code;
+      }
+    }
+  }
+  if (!T) return;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const uint32_t code = scale_code(col_top[e], p.top);
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = x[u].at(e);
+    turned[(c8 + e) * 16 + ((t >> 4) ^ (t & 15))] = f8_eight(v, scale_inverse(code), p.top);
+    if (t < 16 && c8 + e < nc && (GROUP == 1 || c8 + e == 0)) p.st[(GROUP == 1 ? c0 + c8 + e : bj) * p.ldst + bi] = (uint8_t) code;
   }
   __syncthreads();
-  const int line = t >> 1, h = (t & 1) * 64;
-  uint32_t whole = 0;
-  if (GROUP == 128) {
-    uint32_t m = 0;
-    for (int e = 0; e < 64; e++) m = max(m, finite_magnitude(tile[line][h + e]));
-    top[t] = m;
-    __syncthreads();
-    for (int e = 0; e < 256; e++) whole = max(whole, top[e]);
-    __syncthreads();
-  }
-  for (int pass = 0; pass < 2; pass++) {   // 0: rows of X, 1: its columns
-    uint8_t *q = pass ? p.qt : p.q, *s = pass ? p.st : p.s;
-    if (!q) continue;
-    const int64_t ld = pass ? p.ldqt : p.ldq, lds = pass ? p.ldst : p.lds;
-    const int64_t line0 = pass ? c0 : r0, along0 = pass ? r0 : c0, block = pass ? bi : bj;
-    const int lines = pass ? nc : nr, along = pass ? nr : nc;
-    uint32_t m = whole;
-    if (GROUP == 1) {
-      m = 0;
-      for (int e = 0; e < 64; e++) m = max(m, finite_magnitude(pass ? tile[h + e][line] : tile[line][h + e]));
-      m = max(m, (uint32_t) __shfl_xor((int) m, 1));
-    }
-    const uint32_t code = scale_code<F8>(m);
-    const float inv = scale_inverse(code);
-    if (line < lines) {
-      if (h == 0 && (GROUP == 1 || line == 0)) s[(line0 + line) / GROUP * lds + block] = (uint8_t) code;
-      for (int e = 0; e < 64 && h + e < along; e++) {
-        const float v = pass ? tile[h + e][line] : tile[line][h + e];
-        q[(line0 + line) * ld + along0 + h + e] = (uint8_t) f8_pair<F8, false>(v * inv, 0.f, 0u);
-      }
+#pragma unroll
+  for (int u = 0; u < 4; u++) {   // 8 threads a column: two units each
+    const int c = u * 32 + (t >> 3), k = c >> 3, pair = t & 7;
+    if (c >= nc) continue;
+    uint8_t *to = p.qt + (c0 + c) * p.ldqt + r0 + pair * 16;
+    const uint64_t lo = turned[c * 16 + ((2 * pair) ^ k)], hi = turned[c * 16 + ((2 * pair + 1) ^ k)];
+    if (pair * 16 + 16 <= nr) {
+      const uint64_t both[2] = {lo, hi};
+      __builtin_memcpy(to, both, 16);
+    } else {
+      store_bytes(to, lo, nr - pair * 16);
+      store_bytes(to + 8, hi, nr - pair * 16 - 8);
     }
   }
 }
 
-template <int X, int F8>
+template <int X>
 hipError_t launch_quant(const Quant &p, int group, hipStream_t st) {
   const unsigned tiles = (unsigned) (((p.rows + 127) >> 7) * ((p.cols + 127) >> 7));
   drop_stale_error();
-  if (group == 1) quant_tile_kernel<X, F8, 1><<<tiles, 256, 0, st>>>(p);
-  else quant_tile_kernel<X, F8, 128><<<tiles, 256, 0, st>>>(p);
+  if (p.qt) {
+    if (group == 1) quant_kernel<X, 1, true><<<tiles, 256, 0, st>>>(p);
+    else quant_kernel<X, 128, true><<<tiles, 256, 0, st>>>(p);
+  } else {
+    if (group == 1) quant_kernel<X, 1, false><<<tiles, 256, 0, st>>>(p);
+    else quant_kernel<X, 128, false><<<tiles, 256, 0, st>>>(p);
+  }
   return hipGetLastError();
+}
+
+// ---- a row and its team -------------------------------------------------------------
+// TEAM threads (a wave, or a workgroup of several) work on one row; thread t of the team holds CH chunks of eight
+// neighbours, chunk i at column (i * TEAM + t) * 8: 16 neighbouring lanes hold one block of 128.  Rows of up to
+// TEAM * CH * 8 columns stay in registers (KEEP); longer ones are read again for the second half of the work.
+constexpr int team_width(int team, int ch) { return team * ch * 8; }
+
+// sum over the team, in a fixed order, for all of it; `part`: a float for each wave of the workgroup
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float *part) {
+  v = sum_of_wave(v);
+  if constexpr (TEAM > 64) {
+    __syncthreads();   // (the last sum's parts have been read)
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < TEAM / 64; i++) v += part[i];
+  }
+  return v;
 }
 
 // ---- norm ---------------------------------------------------------------------------
 struct Norm {
   const void *x, *r, *w;
-  int64_t ldx, ldr, ldh, ldq, lds, ldy, n;
+  int64_t ldx, ldr, ldh, ldq, lds, ldy, n, rows;
   float eps;
   void *h, *y;
   uint8_t *q, *s;
   float *rstd;
+  int top;
 };
 
-// sum over the workgroup's 256 threads, in a fixed order, for all of them
-__device__ __forceinline__ float group_sum(float v, float *part) {
+template <int T, int TEAM, int CH, bool KEEP>
+__global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_kernel(Norm p) {
+  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+  __shared__ float part[TEAM < 256 ? 1 : TEAM / 64];
+  const int t = threadIdx.x % TEAM;
+  const int64_t row = (int64_t) blockIdx.x * TEAMS + threadIdx.x / TEAM;
+  if (TEAMS > 1 && row >= p.rows) return;
+  float h[CH][8];
+  auto fetch = [&](int64_t c0) {
+    Eight<T> x[CH], r[CH];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = (part[0] + part[1]) + (part[2] + part[3]);
-  __syncthreads();
-  return v;
-}
-
-// One workgroup a row, which is read twice.
-template <int T, int F8>
-__global__ void __launch_bounds__(256) norm_row_kernel(Norm p) {
-  __shared__ float part[4];
-  const int64_t row = blockIdx.x;
-  const int t = threadIdx.x;
+    for (int i = 0; i < CH; i++) {
+      const int64_t c = c0 + (i * TEAM + t) * 8;
+      x[i] = load_eight<T>(p.x, row * p.ldx + c, p.n - c);
+      if (p.r) r[i] = load_eight<T>(p.r, row * p.ldr + c, p.n - c);
+    }
+#pragma unroll
+    for (int i = 0; i < CH; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) h[i][e] = p.r ? x[i].at(e) + r[i].at(e) : x[i].at(e);
+  };
   float sq = 0.f;
-  for (int64_t c = t; c < p.n; c += 256) {
-    float v = load_dense<T>(p.x, row * p.ldx + c);
-    if (p.r) v += load_dense<T>(p.r, row * p.ldr + c);
-    sq = fmaf(v, v, sq);
+  for (int64_t c0 = 0; c0 < (KEEP ? 1 : p.n); c0 += team_width(TEAM, CH)) {
+    fetch(c0);
+#pragma unroll
+    for (int i = 0; i < CH; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) sq = fmaf(h[i][e], h[i][e], sq);
   }
-  const float rstd = 1.f / sqrtf(group_sum(sq, part) / (float) p.n + p.eps);
+  const float rstd = 1.f / sqrtf(team_sum<TEAM>(sq, part) / (float) p.n + p.eps);
   if (t == 0 && p.rstd) p.rstd[row] = rstd;
-  for (int64_t c0 = 0; c0 < p.n; c0 += 512) {   // a wave: one block of 128, two neighbours a lane
-    const int64_t c = c0 + 2 * t;
-    float y[2] = {0.f, 0.f};
-    uint32_t m = 0;
-    for (int e = 0; e < 2; e++)
-      if (c + e < p.n) {
-        float v = load_dense<T>(p.x, row * p.ldx + c + e);
-        if (p.r) v += load_dense<T>(p.r, row * p.ldr + c + e);
-        if (p.h) store_dense<T>(p.h, row * p.ldh + c + e, v);
-        y[e] = v * rstd * load_dense<T>(p.w, c + e);
-        if (p.y) store_dense<T>(p.y, row * p.ldy + c + e, y[e]);
+  for (int64_t c0 = 0; c0 < (KEEP ? 1 : p.n); c0 += team_width(TEAM, CH)) {
+    if (!KEEP) fetch(c0);
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int64_t c = c0 + (i * TEAM + t) * 8, valid = p.n - c;
+      if (p.h) store_eight<T>(p.h, row * p.ldh + c, h[i], valid);
+      if (!p.y && !p.q) continue;
+      const Eight<T> w = load_eight<T>(p.w, c, valid);
+      float y[8];
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        y[e] = e < valid ? h[i][e] * rstd * w.at(e) : 0.f;   // (rstd may be infinite: nothing beyond the row counts)
         m = max(m, finite_magnitude(y[e]));
       }
-    if (!p.q) continue;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t) __shfl_xor((int) m, d));
-    const uint32_t code = scale_code<F8>(m), two = f8_pair<F8, false>(y[0] * scale_inverse(code), y[1] * scale_inverse(code), 0u);
-    for (int e = 0; e < 2; e++)
-      if (c + e < p.n) p.q[row * p.ldq + c + e] = (uint8_t) (two >> (8 * e));
-    if ((t & 63) == 0 && c < p.n) p.s[row * p.lds + (c >> 7)] = (uint8_t) code;
+      if (p.y) store_eight<T>(p.y, row * p.ldy + c, y, valid);
+      if (p.q) {
+        const uint32_t code = scale_code(max_of_16(m), p.top);
+        store_bytes(p.q + row * p.ldq + c, f8_eight(y, scale_inverse(code), p.top), valid);
+        if ((t & 15) == 0 && valid > 0) p.s[row * p.lds + (c >> 7)] = (uint8_t) code;
+      }
+    }
   }
+}
+
+template <int T, int TEAM, int CH, bool KEEP = true>
+void start_norm(const Norm &p, hipStream_t st) {
+  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+  norm_kernel<T, TEAM, CH, KEEP><<<(unsigned) ((p.rows + TEAMS - 1) / TEAMS), TEAM < 256 ? 256 : TEAM, 0, st>>>(p);
+}
+template <int T>
+hipError_t launch_norm(const Norm &p, hipStream_t st) {
+  drop_stale_error();
+  if (p.n <= team_width(64, 1)) start_norm<T, 64, 1>(p, st);
+  else if (p.n <= team_width(64, 2)) start_norm<T, 64, 2>(p, st);
+  else if (p.n <= team_width(256, 1)) start_norm<T, 256, 1>(p, st);
+  else if (p.n <= team_width(256, 2)) start_norm<T, 256, 2>(p, st);
+  else if (p.n <= team_width(256, 4)) start_norm<T, 256, 4>(p, st);
+  else if (p.n <= team_width(1024, 2)) start_norm<T, 1024, 2>(p, st);
+  else if (p.n <= team_width(1024, 4)) start_norm<T, 1024, 4>(p, st);
+  else start_norm<T, 1024, 4, false>(p, st);
+  return hipGetLastError();
 }
 
 // ---- gradient of the norm -----------------------------------------------------------
@@ -137,59 +235,136 @@ struct NormGrad {
   const float *rstd;
   void *dx;
   int64_t lddy, ldh, lddh, lddx, rows, n;
-  float *part, *dw;   // part: gridDim.x rows of n
+  float *part;   // a row of n sums for each team
+  float *dw;
   float beta;
+  int teams;
 };
 
-// Workgroup g of G takes rows g, g + G, ...: dx row by row, and the sums over its rows into part[g].
-template <int T>
-__global__ void __launch_bounds__(256) norm_grad_kernel(NormGrad p) {
-  __shared__ float red[4];
-  float *part = p.part ? p.part + (int64_t) blockIdx.x * p.n : nullptr;
-  const int t = threadIdx.x;
-  bool first = true;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+// Team g of `teams` takes rows g, g + teams, ...: every thread keeps its columns' part of dw in registers over all of them
+// (rows too long for that: in the team's row of `part`).
+template <int T, int TEAM, int CH, bool KEEP>
+__global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_grad_kernel(NormGrad p) {
+  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+  __shared__ float red[TEAM < 256 ? 1 : TEAM / 64];
+  const int t = threadIdx.x % TEAM, team = blockIdx.x * TEAMS + threadIdx.x / TEAM;
+  if (TEAMS > 1 && team >= p.teams) return;
+  float *part = p.part ? p.part + (int64_t) team * p.n : nullptr;
+  const int64_t span = KEEP ? 1 : p.n;
+  float dw[CH][8] = {};
+  Eight<T> w[CH], dy[CH], h[CH], dh[CH];
+  auto fetch = [&](int64_t row, int64_t c0) {
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int64_t c = c0 + (i * TEAM + t) * 8;
+      dy[i] = load_eight<T>(p.dy, row * p.lddy + c, p.n - c);
+      h[i] = load_eight<T>(p.h, row * p.ldh + c, p.n - c);
+      if (p.dh && KEEP) dh[i] = load_eight<T>(p.dh, row * p.lddh + c, p.n - c);
+      if (!KEEP) w[i] = load_eight<T>(p.w, c, p.n - c);
+    }
+  };
+  if (KEEP) {
+#pragma unroll
+    for (int i = 0; i < CH; i++) w[i] = load_eight<T>(p.w, (i * TEAM + t) * 8, p.n - (i * TEAM + t) * 8);
+  }
+  for (int64_t row = team; row < p.rows; row += p.teams) {
     const float rstd = p.rstd[row];
     float dot = 0.f;
-    for (int64_t c = t; c < p.n; c += 256)
-      dot = fmaf(load_dense<T>(p.dy, row * p.lddy + c) * load_dense<T>(p.w, c), load_dense<T>(p.h, row * p.ldh + c) * rstd, dot);
-    const float mean = group_sum(dot, red) / (float) p.n;
-    for (int64_t c = t; c < p.n; c += 256) {
-      const float dy = load_dense<T>(p.dy, row * p.lddy + c), xhat = load_dense<T>(p.h, row * p.ldh + c) * rstd;
-      float v = rstd * (dy * load_dense<T>(p.w, c) - xhat * mean);
-      if (p.dh) v += load_dense<T>(p.dh, row * p.lddh + c);
-      store_dense<T>(p.dx, row * p.lddx + c, v);
-      if (part) part[c] = first ? dy * xhat : part[c] + dy * xhat;
+    for (int64_t c0 = 0; c0 < span; c0 += team_width(TEAM, CH)) {
+      fetch(row, c0);
+#pragma unroll
+      for (int i = 0; i < CH; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) dot = fmaf(dy[i].at(e) * w[i].at(e), h[i].at(e) * rstd, dot);
     }
-    first = false;
+    const float mean = team_sum<TEAM>(dot, red) / (float) p.n;
+    for (int64_t c0 = 0; c0 < span; c0 += team_width(TEAM, CH)) {
+      if (!KEEP) fetch(row, c0);
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const int64_t c = c0 + (i * TEAM + t) * 8, valid = p.n - c;
+        if (!KEEP && p.dh) dh[i] = load_eight<T>(p.dh, row * p.lddh + c, valid);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float g = dy[i].at(e), xhat = h[i].at(e) * rstd;
+          v[e] = rstd * (g * w[i].at(e) - xhat * mean);
+          if (p.dh) v[e] += dh[i].at(e);
+          if (KEEP) dw[i][e] += g * xhat;
+        }
+        store_eight<T>(p.dx, row * p.lddx + c, v, valid);
+        if (!KEEP && part) {
+          const bool first = row == team;
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (e < valid) {
+              const float g = dy[i].at(e) * (h[i].at(e) * rstd);
+              part[c + e] = first ? g : part[c + e] + g;
+            }
+        }
+      }
+    }
+  }
+  if (KEEP && part) {
+#pragma unroll
+    for (int i = 0; i < CH; i++) store_eight<BOF_F32>(part, (i * TEAM + t) * 8, dw[i], p.n - (i * TEAM + t) * 8);
   }
 }
 
-// dw = beta * dw + the partial sums, in their order
-__global__ void __launch_bounds__(256) norm_grad_join_kernel(const float *part, int parts, int64_t n, float beta, float *dw) {
-  const int64_t c = (int64_t) blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  float sum = 0.f;
-  for (int g = 0; g < parts; g++) sum += part[g * n + c];
-  dw[c] = beta == 0.f ? sum : fmaf(beta, dw[c], sum);
+// dw = beta * dw + the teams' sums.  A workgroup: 64 columns, four a thread; 16 slices of the teams, each summed in its order,
+// then the slices in theirs.
+__global__ void __launch_bounds__(256) norm_grad_join_kernel(const float *part, int teams, int64_t n, float beta, float *dw) {
+  __shared__ f32x4 sums[16][16];
+  const int t = threadIdx.x, col = t & 15, slice = t >> 4;
+  const int64_t c = (int64_t) blockIdx.x * 64 + col * 4;
+  const int per = (teams + 15) / 16, g0 = slice * per, g1 = min(teams, g0 + per);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (c + 4 <= n) {
+#pragma unroll 8
+    for (int g = g0; g < g1; g++) {
+      f32x4 v;
+      __builtin_memcpy(&v, part + g * n + c, 16);
+      sum += v;
+    }
+  } else {
+    for (int g = g0; g < g1; g++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (c + e < n) sum[e] += part[g * n + c + e];
+  }
+  sums[slice][col] = sum;
+  __syncthreads();
+  if (t >= 64) return;
+  const int64_t to = (int64_t) blockIdx.x * 64 + t;
+  if (to >= n) return;
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) v += sums[i][t >> 2][t & 3];
+  dw[to] = beta == 0.f ? v : fmaf(beta, dw[to], v);
 }
 
-constexpr int64_t kGradGroups = 256;
-
-template <int T>
-hipError_t launch_norm(const Norm &p, int64_t rows, int f8_type, hipStream_t st) {
-  drop_stale_error();
-  if (f8_type == BOF_E5M2) norm_row_kernel<T, BOF_E5M2><<<(unsigned) rows, 256, 0, st>>>(p);
-  else norm_row_kernel<T, BOF_E4M3><<<(unsigned) rows, 256, 0, st>>>(p);
-  return hipGetLastError();
+// enough teams to fill the card; each writes a row of n sums, which the join reads: 3 % of the rows' own bytes at 8192 rows
+int64_t grad_teams(int64_t rows, int64_t n) {
+  const int64_t most = n <= team_width(64, 2) ? 2048 : n <= team_width(256, 4) ? 512 : 256;
+  return rows < most ? rows : most;
 }
 
+template <int T, int TEAM, int CH, bool KEEP = true>
+void start_norm_grad(const NormGrad &p, hipStream_t st) {
+  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+  norm_grad_kernel<T, TEAM, CH, KEEP><<<(unsigned) ((p.teams + TEAMS - 1) / TEAMS), TEAM < 256 ? 256 : TEAM, 0, st>>>(p);
+}
 template <int T>
 hipError_t launch_norm_grad(const NormGrad &p, hipStream_t st) {
-  const int64_t groups = p.rows < kGradGroups ? p.rows : kGradGroups;
   drop_stale_error();
-  norm_grad_kernel<T><<<(unsigned) groups, 256, 0, st>>>(p);
-  if (p.dw) norm_grad_join_kernel<<<(unsigned) ((p.n + 255) / 256), 256, 0, st>>>(p.part, (int) groups, p.n, p.beta, p.dw);
+  if (p.n <= team_width(64, 1)) start_norm_grad<T, 64, 1>(p, st);
+  else if (p.n <= team_width(64, 2)) start_norm_grad<T, 64, 2>(p, st);
+  else if (p.n <= team_width(256, 1)) start_norm_grad<T, 256, 1>(p, st);
+  else if (p.n <= team_width(256, 2)) start_norm_grad<T, 256, 2>(p, st);
+  else if (p.n <= team_width(256, 4)) start_norm_grad<T, 256, 4>(p, st);
+  else if (p.n <= team_width(1024, 2)) start_norm_grad<T, 1024, 2>(p, st);
+  else start_norm_grad<T, 1024, 1, false>(p, st);
+  if (p.dw) norm_grad_join_kernel<<<(unsigned) ((p.n + 63) / 64), 256, 0, st>>>(p.part, p.teams, p.n, p.beta, p.dw);
   return hipGetLastError();
 }
 
@@ -221,14 +396,9 @@ int bof_f8_quant(int64_t rows, int64_t cols, const void *x, int64_t ldx, int x_t
   if (dev.status()) return dev.status();
   for (auto [p, name] : {std::pair<const void *, const char *>{x, "X"}, {q, "q"}, {s, "s"}, {qt, "qt"}, {st, "st"}})
     if (int rc = p ? dev.reaches(p, kCall, name) : 0) return rc;
-  Quant p{x, ldx, rows, cols, (uint8_t *) q, s, (uint8_t *) qt, st, ldq, lds, ldqt, ldst};
+  Quant p{x, ldx, rows, cols, (uint8_t *) q, s, (uint8_t *) qt, st, ldq, lds, ldqt, ldst, f8_top(f8_type)};
   hipStream_t hs = (hipStream_t) stream;
-  hipError_t e;
-  if (f8_type == BOF_E4M3)
-    e = x_type == BOF_F32 ? launch_quant<BOF_F32, BOF_E4M3>(p, group, hs) : x_type == BOF_BF16 ? launch_quant<BOF_BF16, BOF_E4M3>(p, group, hs) : launch_quant<BOF_F16, BOF_E4M3>(p, group, hs);
-  else
-    e = x_type == BOF_F32 ? launch_quant<BOF_F32, BOF_E5M2>(p, group, hs) : x_type == BOF_BF16 ? launch_quant<BOF_BF16, BOF_E5M2>(p, group, hs) : launch_quant<BOF_F16, BOF_E5M2>(p, group, hs);
-  BOF_HIP_TRY(e);
+  BOF_HIP_TRY(x_type == BOF_F32 ? launch_quant<BOF_F32>(p, group, hs) : x_type == BOF_BF16 ? launch_quant<BOF_BF16>(p, group, hs) : launch_quant<BOF_F16>(p, group, hs));
   return BOF_OK;
 }
 
@@ -252,15 +422,15 @@ int bof_rmsnorm_f8(int64_t rows, int64_t n, int type, const void *x, int64_t ldx
   if (dev.status()) return dev.status();
   for (auto [p, name] : {std::pair<const void *, const char *>{x, "X"}, {r, "R"}, {w, "w"}, {h, "h"}, {q, "q"}, {s, "s"}, {y, "y"}, {rstd, "rstd"}})
     if (int rc = p ? dev.reaches(p, kCall, name) : 0) return rc;
-  Norm p{x, r, w, ldx, ldr, ldh, ldq, lds, ldy, n, eps, h, y, (uint8_t *) q, s, rstd};
+  Norm p{x, r, w, ldx, ldr, ldh, ldq, lds, ldy, n, rows, eps, h, y, (uint8_t *) q, s, rstd, f8_top(f8_type)};
   hipStream_t hs = (hipStream_t) stream;
-  BOF_HIP_TRY(type == BOF_F32 ? launch_norm<BOF_F32>(p, rows, f8_type, hs) : type == BOF_BF16 ? launch_norm<BOF_BF16>(p, rows, f8_type, hs) : launch_norm<BOF_F16>(p, rows, f8_type, hs));
+  BOF_HIP_TRY(type == BOF_F32 ? launch_norm<BOF_F32>(p, hs) : type == BOF_BF16 ? launch_norm<BOF_BF16>(p, hs) : launch_norm<BOF_F16>(p, hs));
   return BOF_OK;
 }
 
 uint64_t bof_rmsnorm_grad_workspace_bytes(int64_t rows, int64_t n) {
   if (rows <= 0 || n <= 0 || rows > (1 << 24) - 1 || n > INT32_MAX - 255) return 0;
-  return (uint64_t) (rows < kGradGroups ? rows : kGradGroups) * (uint64_t) n * 4u;
+  return (uint64_t) grad_teams(rows, n) * (uint64_t) n * 4u;
 }
 
 int bof_rmsnorm_grad(int64_t rows, int64_t n, int type, const void *dy, int64_t lddy, const void *h, int64_t ldh, const void *w,
@@ -288,13 +458,13 @@ int bof_rmsnorm_grad(int64_t rows, int64_t n, int type, const void *dy, int64_t 
   if (int rc = dw ? dev.reaches(dw, kCall, "dw") : 0) return rc;
   if (rows == 0) {   // no rows: dw = beta * dw
     drop_stale_error();
-    norm_grad_join_kernel<<<(unsigned) ((n + 255) / 256), 256, 0, hs>>>(nullptr, 0, n, beta, dw);
+    norm_grad_join_kernel<<<(unsigned) ((n + 63) / 64), 256, 0, hs>>>(nullptr, 0, n, beta, dw);
     BOF_HIP_TRY(hipGetLastError());
     return BOF_OK;
   }
   for (auto [p, name] : {std::pair<const void *, const char *>{dy, "dy"}, {h, "h"}, {w, "w"}, {rstd, "rstd"}, {dh, "dh"}, {dx, "dx"}, {dw ? work : nullptr, "work"}})
     if (int rc = p ? dev.reaches(p, kCall, name) : 0) return rc;
-  NormGrad p{dy, h, w, dh, rstd, dx, lddy, ldh, lddh, lddx, rows, n, dw ? (float *) work : nullptr, dw, beta};
+  NormGrad p{dy, h, w, dh, rstd, dx, lddy, ldh, lddh, lddx, rows, n, dw ? (float *) work : nullptr, dw, beta, (int) grad_teams(rows, n)};
   BOF_HIP_TRY(type == BOF_F32 ? launch_norm_grad<BOF_F32>(p, hs) : type == BOF_BF16 ? launch_norm_grad<BOF_BF16>(p, hs) : launch_norm_grad<BOF_F16>(p, hs));
   return BOF_OK;
 }
