@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(256) f8_tile_any_kernel(F8Product p) {
   const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
   const int l16 = lane & 15, g = lane >> 4;
   const int nb = (p.k + 127) >> 7;
-  const int b0 = blockIdx.y * p.blocks_per_part, b1 = min(nb, b0 + p.blocks_per_part);
+  const int b0 = blockIdx.y * p.blocks_per_part, b1 = blockIdx.y == gridDim.y - 1 ? nb : b0 + p.blocks_per_part;
   f32x4 acc[4][4];
 #pragma unroll
   for (int x = 0; x < 16; x++) acc[x >> 2][x & 3] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -198,25 +198,27 @@ __global__ void __launch_bounds__(256) f8_tile_any_kernel(F8Product p) {
       }
 }
 
-// ---- 256 x 256 tiles ----------------------------------------------------------------
-// Four waves, one on each SIMD, 128 x 128 of C each: 64 accumulators of four floats = 256 registers (the accumulator
-// half of the file), the other half holds the fragments.  A slab is one block of k, 256 rows x 128 bytes of each operand;
-// both lie in LDS twice (128 KB).  Rows reach LDS without touching registers: one global_load_lds_dwordx4 moves 8 rows,
-// lane l fetching chunk (l & 7) ^ (l >> 3) of row l >> 3, so that the image is [row][chunk ^ (row & 7)] and a fragment
-// read (16 rows x 16 bytes) meets every bank once.  Per slab and wave: 64 MFMAs of 32 cycles, 32 ds_read_b128, 16 DMA
-// pieces.
+// ---- tiles ---------------------------------------------------------------------------
+// Four waves, X x Y tiles of 16 x 16 each, 2 x 2 waves: a workgroup owns 32 X rows and 32 Y columns of C.  8 x 8 (256 x 256):
+// one wave on each SIMD, 64 accumulators of four floats = 256 registers (the accumulator half of the file), the other half
+// holds the fragments.  4 x 4 (128 x 128): two workgroups a CU, for outputs with few tiles.
 //
-// The A fragments of a slab are read into registers during the slab BEFORE (8 x 8 registers, twice), the B fragments one
-// tile ahead.  The barrier of a slab stands in front of its last B tile: by then every wave has read all it wants from
-// this slab's B image and the next slab's A image, and the pieces of the next B and the next but one A image, issued at the
-// slab's start, have landed.
+// A slab is one block of k: rows of 128 bytes; both operands lie in LDS twice.  DMA: rows reach LDS without touching
+// registers -- one global_load_lds_dwordx4 moves 8 rows, lane l fetching chunk (l & 7) ^ (l >> 3) of row l >> 3, so that the
+// image is [row][chunk ^ (row & 7)] and a fragment read (16 rows x 16 bytes) meets every bank once.  It needs rows aligned to
+// 16 bytes; for others (DMA = false) a thread loads its 16-byte chunks of the same rows, unaligned, and writes them to the
+// same places one slab later.  Per slab and wave of 8 x 8: 64 MFMAs of 32 cycles, 32 ds_read_b128, 16 pieces.
 //
-// Scales: thread t fetches the word with four blocks' scales of A row t and of B row t, once in four slabs, into LDS
-// (twice 2 KB); a fragment's scale byte is read from there along with it.  No vector instruction is left in a slab but a few
-// for the whole of it.
+// The A fragments of a slab are read into registers during the slab BEFORE (twice X x 8 registers), the B fragments one tile
+// ahead.  The barrier of a slab stands in front of its last row of tiles: by then every wave has read all it wants from this
+// slab's B image and the next slab's A image, and the pieces of the next B and the next but one A image, issued at the slab's
+// start, have landed.
 //
-// A tile at the lower or right edge starts earlier (at m - 256, n - 256), so that every row it fetches exists; what lies
-// in the tile before is not stored again.
+// Scales: a thread fetches the word with four blocks' scales of its rows, once in four slabs, into LDS (twice); a fragment's
+// scale byte is read from there along with it.  No vector instruction is left in a slab but a few for the whole of it.
+//
+// A tile at the lower or right edge starts earlier (at m - 32 X, n - 32 Y), so that every row it fetches exists; what lies in
+// the tile before is not stored again.
 __device__ __forceinline__ uint32_t lds_address(const void *p) {
   return (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) void *) p;
 }
@@ -237,215 +239,290 @@ __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int g
   tn = bid % per / deep;
 }
 
-// The four scale bytes of blocks b .. b + 3 of a row (nb >= 4 blocks in all, b < nb) as one word, read inside the row:
-// the word that is read begins up to three bytes early, scale_shift bits of it are left out.
+// The four scale bytes of blocks b .. b + 3 of a row of nb > b as one word, read inside the row: the word that is read begins
+// up to three bytes early, scale_shift bits of it are left out (rows of fewer than four bytes are read byte by byte).
 __device__ __forceinline__ uint32_t scale_word(const uint8_t *row, int b, int nb) {
   uint32_t w;
-  __builtin_memcpy(&w, row + min(b, nb - 4), 4);
+  if (nb >= 4) {
+    __builtin_memcpy(&w, row + min(b, nb - 4), 4);
+  } else {
+    w = row[0];
+    if (nb > 1) w |= (uint32_t) row[1] << 8;
+    if (nb > 2) w |= (uint32_t) row[2] << 16;
+  }
   return w;
 }
-__device__ __forceinline__ int scale_shift(int b, int nb) { return 8 * max(0, b - (nb - 4)); }
+__device__ __forceinline__ int scale_shift(int b, int nb) { return 8 * max(0, b - max(nb - 4, 0)); }
 
 __device__ __forceinline__ i32x8 both(u32x4 lo, u32x4 hi) {
   return i32x8{(int) lo[0], (int) lo[1], (int) lo[2], (int) lo[3], (int) hi[0], (int) hi[1], (int) hi[2], (int) hi[3]};
 }
 
-// A wave's 128 x 128 sums to C, from row i, column j on: 64 rows at a time through the wave's own 32 KB of LDS (rows of
-// 32 chunks of four floats, XOR-ed with the row), so that a row of C leaves in whole lines.  Rows before i_from and
-// columns before j_from are left out.
-__device__ __forceinline__ void store_wave_128(const F8Product &p, f32x4 (&acc)[8][8], f32x4 *own, int i, int j, int i_from, int j_from) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const bool wide = p.c_type != BOF_F32 && p.beta == 0.f && p.ldc % 8 == 0 && j_from == j && j + 128 <= p.n && j % 8 == 0 && reinterpret_cast<uintptr_t>(p.c) % 16 == 0;
+// alpha * v + beta * C of eight neighbours that all lie inside C
+template <int T>
+__device__ __forceinline__ void finish_eight(const F8Product &p, int64_t at, f32x4 lo, f32x4 hi) {
+  float v[8];
 #pragma unroll
-  for (int half = 0; half < 2; half++) {
+  for (int e = 0; e < 8; e++) v[e] = p.alpha * (e < 4 ? lo[e] : hi[e - 4]);
+  if (p.beta != 0.f) {
+    const Eight<T> c = load_eight<T>(p.c, at, 8);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = fmaf(p.beta, c.at(e), v[e]);
+  }
+  store_eight<T>(p.c, at, v, 8);
+}
+
+// A wave's sums to C, from row i, column j on: 64 rows at a time through the wave's own part of LDS (rows of 4 Y chunks of four
+// floats, XOR-ed with the row), so that a row of C leaves in whole lines.  Rows before i_from and columns before j_from are left
+// out.
+template <int X, int Y>
+__device__ __forceinline__ void store_wave(const F8Product &p, f32x4 (&acc)[X][Y], f32x4 *own, int i, int j, int i_from, int j_from) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  constexpr int W = 4 * Y, LANES = 2 * Y;   // chunks in a row, lanes a row
+#pragma unroll
+  for (int part = 0; part < X / 4; part++) {
 #pragma unroll
     for (int x = 0; x < 4; x++)
 #pragma unroll
-      for (int y = 0; y < 8; y++) own[(x * 16 + l16) * 32 + ((y * 4 + g) ^ (l16 & 7))] = acc[half * 4 + x][y];
+      for (int y = 0; y < Y; y++) own[(x * 16 + l16) * W + ((y * 4 + g) ^ (l16 & 7))] = acc[part * 4 + x][y];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (wide) {
-#pragma unroll 4
-      for (int it = 0; it < 16; it++) {
-        const int r = it * 4 + g, row = i + half * 64 + r;
-        const f32x4 v0 = own[r * 32 + ((l16 * 2) ^ (r & 7))], v1 = own[r * 32 + ((l16 * 2 + 1) ^ (r & 7))];
-        if (row < i_from || row >= p.m) continue;
-        if (p.c_type == BOF_BF16) {
-          typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-          b8 o;
+#pragma unroll 2
+    for (int it = 0; it < LANES; it++) {
+      const int r = it * (64 / LANES) + lane / LANES, c2 = lane % LANES * 2, row = i + part * 64 + r, col = j + c2 * 4;
+      const f32x4 lo = own[r * W + (c2 ^ (r & 7))], hi = own[r * W + ((c2 + 1) ^ (r & 7))];
+      if (row < i_from || row >= p.m) continue;
+      if (col >= j_from && col + 8 <= p.n) {
+        const int64_t at = (int64_t) row * p.ldc + col;
+        if (p.c_type == BOF_BF16) finish_eight<BOF_BF16>(p, at, lo, hi);
+        else if (p.c_type == BOF_F16) finish_eight<BOF_F16>(p, at, lo, hi);
+        else finish_eight<BOF_F32>(p, at, lo, hi);
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; e++) { o[e] = (__bf16) (p.alpha * v0[e]); o[e + 4] = (__bf16) (p.alpha * v1[e]); }
-          *(b8 *) ((__bf16 *) p.c + (int64_t) row * p.ldc + j + l16 * 8) = o;
-        } else {
-          typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-          h8 o;
-#pragma unroll
-          for (int e = 0; e < 4; e++) { o[e] = (_Float16) (p.alpha * v0[e]); o[e + 4] = (_Float16) (p.alpha * v1[e]); }
-          *(h8 *) ((_Float16 *) p.c + (int64_t) row * p.ldc + j + l16 * 8) = o;
-        }
-      }
-    } else {
-#pragma unroll 1
-      for (int it = 0; it < 128; it++) {
-        const int r = it >> 1, c = (it & 1) * 64 + lane, row = i + half * 64 + r;
-        const float v = ((const float *) own)[(r * 32 + ((c >> 2) ^ (r & 7))) * 4 + (c & 3)];
-        if (row >= i_from && row < p.m && j + c >= j_from && j + c < p.n) finish(p, row, j + c, v);
+        for (int e = 0; e < 8; e++)
+          if (col + e >= j_from && col + e < p.n) finish(p, row, col + e, e < 4 ? lo[e] : hi[e - 4]);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
-// The slab's product, its accumulators pinned to the accumulator registers (left to itself the compiler moves them through
-// both halves of the file: 200 copies a slab).  Hazards: the same accumulator comes round after 64 of these, the fragments
-// come from LDS; whoever reads acc afterwards calls settle() first.
-template <int TA, int TB>
+// The slab's product, its accumulators pinned (left to itself the compiler moves them through both halves of the register
+// file: 200 copies a slab): to the accumulator half where they are 256, else to the other.  Hazards: the same accumulator
+// comes round after 16 of these at least, the fragments come from LDS; whoever reads acc afterwards calls settle() first.
+template <int TA, int TB, bool AGPR>
 __device__ __forceinline__ void mma_pinned(const Frag<false> &b, const Frag<false> &a, f32x4 &acc) {
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
-               : "+a"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
+  if constexpr (AGPR)
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
+                 : "+a"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
+  else
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
+                 : "+v"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
 }
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// LDS, in chunks of 16 bytes: A twice, B twice, scale words twice (A rows, B rows)
-constexpr int kImage = 2048, kScales = 4 * kImage, kLds256 = kScales + 2 * 128;
+// A part of a product that is split along k writes its sums instead of C.
+__device__ __forceinline__ F8Product part_of(F8Product p, int z) {
+  if (p.part) {
+    p.c = p.part + (int64_t) z * p.m * p.n;
+    p.c_type = BOF_F32;
+    p.ldc = p.n;
+    p.alpha = 1.f;
+    p.beta = 0.f;
+  }
+  return p;
+}
 
-struct Slab256 {
+template <int X, int Y, bool DMA>
+struct Slab {
+  static constexpr int A_IMAGE = 256 * X, B_IMAGE = 256 * Y;       // chunks of 16 bytes in an image
+  static constexpr int B0 = 2 * A_IMAGE, S0 = B0 + 2 * B_IMAGE;    // where the B images and the scale words begin
+  static constexpr int WORDS = 32 * (X + Y), CHUNKS = S0 + WORDS / 2;
+  static constexpr int PIECES = X + Y;                             // of 32 rows (8 a wave)
   u32x4 *lds;
-  uint32_t a_voff, b_voff;       // of this lane's row in a piece
-  uint64_t a_step, b_step;       // bytes from piece to piece (32 rows)
-  uint32_t a_to, b_to;           // LDS addresses of this wave's pieces in image 0
+  uint32_t a_voff, b_voff;       // of this thread's row and chunk in a piece
+  uint64_t a_step, b_step;       // bytes from piece to piece
+  uint32_t a_to, b_to;           // LDS addresses of this wave's pieces in image 0 (DMA)
+  int put;                       // this thread's chunk in a piece (staged)
   int a_lo, a_hi, b_lo, b_hi;    // this lane's chunks in the image, of tile 0
   const uint8_t *sa, *sb;        // this lane's scale bytes of tile 0, block 0 of four
+  u32x4 staged[DMA ? 1 : PIECES];
 };
 
-template <int TA, int TB, int P>
-__device__ __forceinline__ void slab256(const Slab256 &s, uint64_t b_next, uint64_t a_next, int sc_b, int sc_a, Frag<false> (&fa)[2][8],
-                                        Frag<false> (&fb)[2], f32x4 (&acc)[8][8]) {
+template <int TA, int TB, int X, int Y, bool DMA, int P>
+__device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64_t a_next, int sc_b, int sc_a, Frag<false> (&fa)[2][X],
+                                     Frag<false> (&fb)[2], f32x4 (&acc)[X][Y]) {
+  using S = Slab<X, Y, DMA>;
+  // piece p: B first, into the other B image; then A, into the image whose fragments are in registers
+  auto piece = [&](int q) {
+    const bool b = q < Y;
+    const int r = b ? q : q - Y;
+    const uint64_t from = b ? b_next + r * s.b_step : a_next + r * s.a_step;
+    if constexpr (DMA) {
+      dma16(b ? s.b_voff : s.a_voff, from, (b ? s.b_to + (P ^ 1) * S::B_IMAGE * 16 : s.a_to + P * S::A_IMAGE * 16) + r * 4096);
+    } else {
+      s.lds[s.put + (b ? S::B0 + (P ^ 1) * S::B_IMAGE : P * S::A_IMAGE) + r * 256] = s.staged[q];
+      __builtin_memcpy(&s.staged[q], reinterpret_cast<const uint8_t *>(from) + (b ? s.b_voff : s.a_voff), 16);
+    }
+  };
+  constexpr int N = X * Y, LAST = N - X;   // MFMAs, those in front of the barrier
 #pragma unroll
-  for (int y = 0; y < 8; y++) {
-    if (y == 7) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  for (int y = 0; y < Y; y++) {
+    if (y == Y - 1) {
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     }
 #pragma unroll
-    for (int x = 0; x < 8; x++) {
-      mma_pinned<TA, TB>(fb[y & 1], fa[P][x], acc[x][y]);
+    for (int x = 0; x < X; x++) {
+      const int at = y * X + x;
+      mma_pinned<TA, TB, X * Y == 64>(fb[y & 1], fa[P][x], acc[x][y]);
       if (x == 1) {   // the next B tile: of this slab, or the next one's first
-        const int at = (y < 7 ? P : P ^ 1) * kImage + (y < 7 ? y + 1 : 0) * 128;
-        fb[(y + 1) & 1].q = both(s.lds[s.b_lo + at], s.lds[s.b_hi + at]);
-        fb[(y + 1) & 1].s = s.sb[(y < 7 ? sc_b : sc_a) + (y < 7 ? y + 1 : 0) * 64];
+        const int from = (y < Y - 1 ? P : P ^ 1) * S::B_IMAGE + (y < Y - 1 ? y + 1 : 0) * 128;
+        fb[(y + 1) & 1].q = both(s.lds[s.b_lo + from], s.lds[s.b_hi + from]);
+        fb[(y + 1) & 1].s = s.sb[(y < Y - 1 ? sc_b : sc_a) + (y < Y - 1 ? y + 1 : 0) * 64];
       }
-      if (y < 4 && (x & 1)) {   // pieces: B first
-        const int piece = y * 4 + (x >> 1);
-        if (piece < 8) dma16(s.b_voff, b_next + piece * s.b_step, s.b_to + (P ^ 1) * kImage * 16 + piece * 4096);
-        else dma16(s.a_voff, a_next + (piece - 8) * s.a_step, s.a_to + P * kImage * 16 + (piece - 8) * 4096);
-      }
-      if (y >= 2 && y < 6 && (x == 3 || x == 6)) {   // the next slab's A fragments
-        const int f = (y - 2) * 2 + (x == 6), at = (P ^ 1) * kImage + f * 128;
-        fa[P ^ 1][f].q = both(s.lds[s.a_lo + at], s.lds[s.a_hi + at]);
+      // the pieces: one behind every second MFMA from the start on (4 x 4: behind every one)
+      constexpr int D = LAST / S::PIECES >= 2 ? 2 : 1;
+      if (at % D == D - 1 && at / D < S::PIECES) piece(at / D);
+      // the next slab's A fragments: X of them between a quarter and three quarters of the slab
+      constexpr int F0 = N / 4, STEP = (LAST - F0 - 2) / X > 4 ? 4 : (LAST - F0 - 2) / X;
+      if (at >= F0 && (at - F0) % STEP == 0 && (at - F0) / STEP < X) {
+        const int f = (at - F0) / STEP, from = (P ^ 1) * S::A_IMAGE + f * 128;
+        fa[P ^ 1][f].q = both(s.lds[s.a_lo + from], s.lds[s.a_hi + from]);
         fa[P ^ 1][f].s = s.sa[sc_a + f * 64];
       }
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+  static_assert(S::PIECES <= LAST, "every piece finds its place in front of the barrier");
 }
 
-template <int TA, int TB>
-__global__ void __launch_bounds__(256, 1) f8_tile256_kernel(F8Product p, int tiles_m, int tiles_n) {
-  __shared__ u32x4 lds[kLds256];
+template <int TA, int TB, int X, int Y, bool DMA>
+__global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product q, int tiles_m, int tiles_n) {
+  using S = Slab<X, Y, DMA>;
+  __shared__ u32x4 lds[S::CHUNKS];
+  const F8Product p = part_of(q, blockIdx.y);
+  constexpr int TM = 32 * X, TN = 32 * Y;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
-  const int i0 = min(tm * 256, p.m - 256), j0 = min(tn * 256, p.n - 256);
+  const int i0 = min(tm * TM, p.m - TM), j0 = min(tn * TN, p.n - TN);
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wi = (wave >> 1) * 128, wj = (wave & 1) * 128;
+  const int wi = (wave >> 1) * 16 * X, wj = (wave & 1) * 16 * Y;
   const int l16 = lane & 15, g = lane >> 4;
-  const int nb = (p.k + 127) >> 7, full = p.k >> 7;
-  Slab256 s;
+  const int nb = (p.k + 127) >> 7, all = p.k >> 7;
+  const int b0 = blockIdx.y * p.blocks_per_part, full = min(all, b0 + p.blocks_per_part);   // slabs b0 .. full - 1, one at least
+  const bool tail = nb > all && blockIdx.y == gridDim.y - 1;
+  S s;
   s.lds = lds;
-  const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) << 4;
+  const int r8 = lane >> 3, chunk = (DMA ? (lane & 7) ^ r8 : lane & 7) << 4;
   s.a_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.lda + chunk;
   s.b_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.ldb + chunk;
   s.a_step = (uint64_t) p.lda * 32;
   s.b_step = (uint64_t) p.ldb * 32;
   s.a_to = lds_address(lds) + wave * 1024;
-  s.b_to = s.a_to + 2 * kImage * 16;
+  s.b_to = s.a_to + S::B0 * 16;
+  s.put = (8 * wave + r8) * 8 + ((lane & 7) ^ r8);
   s.a_lo = (wi + l16) * 8 + (g ^ (l16 & 7)); s.a_hi = (wi + l16) * 8 + ((g + 4) ^ (l16 & 7));
-  s.b_lo = 2 * kImage + (wj + l16) * 8 + (g ^ (l16 & 7)); s.b_hi = 2 * kImage + (wj + l16) * 8 + ((g + 4) ^ (l16 & 7));
-  s.sa = (const uint8_t *) (lds + kScales) + (wi + l16) * 4;
-  s.sb = (const uint8_t *) (lds + kScales + 64) + (wj + l16) * 4;
-  uint32_t *const sw = (uint32_t *) (lds + kScales) + t;
-  const uint8_t *const sa_row = p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa, *const sb_row = p.sb + (int64_t) ((j0 + t) >> p.b_shift) * p.ldsb;
+  s.b_lo = S::B0 + (wj + l16) * 8 + (g ^ (l16 & 7)); s.b_hi = S::B0 + (wj + l16) * 8 + ((g + 4) ^ (l16 & 7));
+  s.sa = (const uint8_t *) (lds + S::S0) + (wi + l16) * 4;
+  s.sb = (const uint8_t *) (lds + S::S0) + (TM + wj + l16) * 4;
+  // scale words: thread t has row t of A (t < TM) and row t of B; with 128 + 128 rows one of them
+  uint32_t *const sw = (uint32_t *) (lds + S::S0) + t;
+  constexpr bool TWO = TM == 256;
+  const uint8_t *const s0_row = t < TM ? p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa : p.sb + (int64_t) ((j0 + t - TM) >> p.b_shift) * p.ldsb;
+  const uint8_t *const s1_row = TWO ? p.sb + (int64_t) ((j0 + min(t, TN - 1)) >> p.b_shift) * p.ldsb : s0_row;
+  auto put_words = [&](int to, uint32_t w0, uint32_t w1, int shift) {
+    sw[to] = w0 >> shift;
+    if (TWO && t < TN) sw[to + TM] = w1 >> shift;
+  };
   const uint64_t a_org = reinterpret_cast<uint64_t>(p.a + (int64_t) i0 * p.lda), b_org = reinterpret_cast<uint64_t>(p.b + (int64_t) j0 * p.ldb);
-  // A of slabs 0 and 1, B of slab 0, the scales of the first four
+  auto a_at = [&](int kb) { return a_org + (uint64_t) min(kb, full - 1) * 128; };   // (behind the last slab: the last one again)
+  auto b_at = [&](int kb) { return b_org + (uint64_t) min(kb, full - 1) * 128; };
+  f32x4 acc[X][Y];
 #pragma unroll
-  for (int q = 0; q < 8; q++) {
-    dma16(s.a_voff, a_org + q * s.a_step, s.a_to + q * 4096);
-    dma16(s.b_voff, b_org + q * s.b_step, s.b_to + q * 4096);
-    dma16(s.a_voff, a_org + 128 + q * s.a_step, s.a_to + kImage * 16 + q * 4096);
+  for (int x = 0; x < X * Y; x++) acc[x / Y][x % Y] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Frag<false> fa[2][X], fb[2];
+  // A of the first two slabs, B of the first (staged: and what the first slab is to write), the scales of its four
+#pragma unroll
+  for (int r = 0; r < X; r++) {
+    if constexpr (DMA) {
+      dma16(s.a_voff, a_at(b0) + r * s.a_step, s.a_to + r * 4096);
+      dma16(s.a_voff, a_at(b0 + 1) + r * s.a_step, s.a_to + S::A_IMAGE * 16 + r * 4096);
+    } else {
+      u32x4 v[2];
+      __builtin_memcpy(&v[0], reinterpret_cast<const uint8_t *>(a_at(b0) + r * s.a_step) + s.a_voff, 16);
+      __builtin_memcpy(&v[1], reinterpret_cast<const uint8_t *>(a_at(b0 + 1) + r * s.a_step) + s.a_voff, 16);
+      __builtin_memcpy(&s.staged[Y + r], reinterpret_cast<const uint8_t *>(a_at(b0 + 2) + r * s.a_step) + s.a_voff, 16);
+      lds[s.put + r * 256] = v[0];
+      lds[s.put + S::A_IMAGE + r * 256] = v[1];
+    }
   }
-  f32x4 acc[8][8];
 #pragma unroll
-  for (int x = 0; x < 64; x++) acc[x >> 3][x & 7] = f32x4{0.f, 0.f, 0.f, 0.f};
-  uint32_t wa = scale_word(sa_row, 0, nb), wb = scale_word(sb_row, 0, nb);
-  sw[0] = wa;
-  sw[256] = wb;
+  for (int r = 0; r < Y; r++) {
+    if constexpr (DMA) {
+      dma16(s.b_voff, b_at(b0) + r * s.b_step, s.b_to + r * 4096);
+    } else {
+      u32x4 v;
+      __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(b_at(b0) + r * s.b_step) + s.b_voff, 16);
+      __builtin_memcpy(&s.staged[r], reinterpret_cast<const uint8_t *>(b_at(b0 + 1) + r * s.b_step) + s.b_voff, 16);
+      lds[s.put + S::B0 + r * 256] = v;
+    }
+  }
+  // words of the first four blocks (b0 is a multiple of four); of the next four: fetched in front of slab 0 of four, in LDS
+  // before the barrier of slab 2, read from slab 3 on
+  put_words((b0 & 4) ? S::WORDS : 0, scale_word(s0_row, b0, nb), scale_word(s1_row, b0, nb), scale_shift(b0, nb));
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  Frag<false> fa[2][8], fb[2];
+  auto byte_of = [](int kb) { return ((kb & 4) ? S::WORDS * 4 : 0) + (kb & 3); };
 #pragma unroll
-  for (int x = 0; x < 8; x++) {
+  for (int x = 0; x < X; x++) {
     fa[0][x].q = both(lds[s.a_lo + x * 128], lds[s.a_hi + x * 128]);
-    fa[0][x].s = s.sa[x * 64];
+    fa[0][x].s = s.sa[byte_of(b0) + x * 64];
   }
   fb[0].q = both(lds[s.b_lo], lds[s.b_hi]);
-  fb[0].s = s.sb[0];
+  fb[0].s = s.sb[byte_of(b0)];
   __syncthreads();
-  // (the pieces behind the last slab fetch the last slab again, into images nobody reads)
-  auto words = [&](int kb) {   // in front of slab kb: the next four blocks' scales, fetched at 0, in LDS before 2's barrier
-    if ((kb & 3) == 0 && kb + 4 < nb) { wa = scale_word(sa_row, kb + 4, nb); wb = scale_word(sb_row, kb + 4, nb); }
-    if ((kb & 3) == 2 && kb + 2 < nb) { uint32_t *to = sw + (~kb & 4) * 128; to[0] = wa >> scale_shift(kb + 2, nb); to[256] = wb >> scale_shift(kb + 2, nb); }
+  uint32_t w0 = 0, w1 = 0;
+  auto words = [&](int kb) {
+    if ((kb & 3) == 0 && kb + 4 < nb) { w0 = scale_word(s0_row, kb + 4, nb); w1 = scale_word(s1_row, kb + 4, nb); }
+    if ((kb & 3) == 2 && kb + 2 < nb) put_words((~kb & 4) ? S::WORDS : 0, w0, w1, scale_shift(kb + 2, nb));
   };
-  auto byte_of = [](int kb) { return (kb & 4) * 512 + (kb & 3); };
-  int kb = 0;
+  int kb = b0;
   for (; kb + 2 <= full; kb += 2) {
     words(kb);
-    slab256<TA, TB, 0>(s, b_org + (uint64_t) min(kb + 1, full - 1) * 128, a_org + (uint64_t) min(kb + 2, full - 1) * 128, byte_of(kb), byte_of(kb + 1), fa, fb, acc);
-    slab256<TA, TB, 1>(s, b_org + (uint64_t) min(kb + 2, full - 1) * 128, a_org + (uint64_t) min(kb + 3, full - 1) * 128, byte_of(kb + 1), byte_of(kb + 2), fa, fb, acc);
+    slab<TA, TB, X, Y, DMA, 0>(s, DMA ? b_at(kb + 1) : b_at(kb + 2), DMA ? a_at(kb + 2) : a_at(kb + 3), byte_of(kb), byte_of(kb + 1), fa, fb, acc);
+    slab<TA, TB, X, Y, DMA, 1>(s, DMA ? b_at(kb + 2) : b_at(kb + 3), DMA ? a_at(kb + 3) : a_at(kb + 4), byte_of(kb + 1), byte_of(kb + 2), fa, fb, acc);
   }
-  if (kb < full) {
-    words(kb);
-    slab256<TA, TB, 0>(s, b_org + (uint64_t) (full - 1) * 128, a_org + (uint64_t) (full - 1) * 128, byte_of(kb), byte_of(kb + 1), fa, fb, acc);
-    kb++;
-  }
+  if (kb < full) slab<TA, TB, X, Y, DMA, 0>(s, b_at(kb), a_at(kb), byte_of(kb), byte_of(kb), fa, fb, acc);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
-  if (nb > full) {   // the short block: through registers, zeros behind k
+  if (tail) {   // the short block: through registers, zeros behind k
 #pragma unroll 1
-    for (int u = 0; u < 8; u++) {
-      const int at = t + 256 * u, r = at >> 3, c = at & 7;
-      lds[r * 8 + (c ^ (r & 7))] = load_chunk(p.a + (int64_t) (i0 + r) * p.lda, full * 128 + c * 16, p.k);
-      lds[2 * kImage + r * 8 + (c ^ (r & 7))] = load_chunk(p.b + (int64_t) (j0 + r) * p.ldb, full * 128 + c * 16, p.k);
-    }
-    sw[0] = sa_row[full];
-    sw[256] = sb_row[full];
+    for (int u = 0; u < X; u++)
+      lds[s.put + u * 256] = load_chunk(p.a + (int64_t) (i0 + 32 * u + 8 * wave + r8) * p.lda, all * 128 + (lane & 7) * 16, p.k);
+#pragma unroll 1
+    for (int u = 0; u < Y; u++)
+      lds[s.put + S::B0 + u * 256] = load_chunk(p.b + (int64_t) (j0 + 32 * u + 8 * wave + r8) * p.ldb, all * 128 + (lane & 7) * 16, p.k);
+    put_words(0, s0_row[all], s1_row[all], 0);
     __syncthreads();
 #pragma unroll
-    for (int x = 0; x < 8; x++) {
+    for (int x = 0; x < X; x++) {
       fa[0][x].q = both(lds[s.a_lo + x * 128], lds[s.a_hi + x * 128]);
       fa[0][x].s = s.sa[x * 64];
     }
 #pragma unroll
-    for (int y = 0; y < 8; y++) {
+    for (int y = 0; y < Y; y++) {
       Frag<false> b;
       b.q = both(lds[s.b_lo + y * 128], lds[s.b_hi + y * 128]);
       b.s = s.sb[y * 64];
 #pragma unroll
-      for (int x = 0; x < 8; x++) mma_pinned<TA, TB>(b, fa[0][x], acc[x][y]);
+      for (int x = 0; x < X; x++) mma_pinned<TA, TB, X * Y == 64>(b, fa[0][x], acc[x][y]);
     }
     __syncthreads();
   }
   settle();
-  store_wave_128(p, acc, (f32x4 *) lds + wave * kImage, i0 + wi, j0 + wj, max(tm * 256, i0 + wi), max(tn * 256, j0 + wj));
+  store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, max(tm * TM, i0 + wi), max(tn * TN, j0 + wj));
 }
 
 // C from the parts of the sums, added in their order (no parts: C = beta * C)
@@ -458,33 +535,49 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
   }
 }
 
+// ---- which kernel --------------------------------------------------------------------
 constexpr int kMaxParts = 32;
 
-// parts along k: enough workgroups to fill the card's 256 compute units twice, each with four blocks at least
+// Parts along k: workgroups of 128 x 128 to give every one of the 256 compute units two, each with eight blocks of k at least
+// (the join reads and writes every part again: it pays for itself from about 24 blocks on).
 int wanted_parts(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128), nb = (k + 127) / 128;
-  int64_t parts = tiles > 0 ? 512 / tiles : 1;
-  if (parts > nb / 4) parts = nb / 4;
+  if (nb < 24) return 1;
+  const int64_t parts = 512 / tiles < nb / 8 ? 512 / tiles : nb / 8;
   return (int) (parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
+}
+
+bool rows_aligned(const F8Product &p) {
+  return p.lda % 16 == 0 && p.ldb % 16 == 0 && reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0;
+}
+
+template <int TA, int TB, int X, int Y>
+void start_tiles(const F8Product &p, int parts, hipStream_t st) {
+  const int tiles_m = (p.m + 32 * X - 1) / (32 * X), tiles_n = (p.n + 32 * Y - 1) / (32 * Y);
+  const dim3 grid((unsigned) (tiles_m * tiles_n), (unsigned) parts);
+  if (rows_aligned(p)) f8_tile_kernel<TA, TB, X, Y, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
+  else f8_tile_kernel<TA, TB, X, Y, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 
 template <int TA, int TB>
 hipError_t launch_product(F8Product p, int parts, hipStream_t st) {
-  const int nb = (p.k + 127) / 128;
-  p.blocks_per_part = (nb + parts - 1) / parts;
-  parts = (nb + p.blocks_per_part - 1) / p.blocks_per_part;
+  // parts begin at multiples of four blocks; the short block is the last part's
+  const int all = p.k < 128 ? 1 : p.k / 128;
+  p.blocks_per_part = ((all + parts - 1) / parts + 3) & ~3;
+  parts = (all + p.blocks_per_part - 1) / p.blocks_per_part;
   if (parts == 1) p.part = nullptr;
-  const int tiles_m = (p.m + 255) / 256, tiles_n = (p.n + 255) / 256;
-  if (p.c_type != BOF_F32 && p.m >= 256 && p.n >= 256 && (int64_t) tiles_m * tiles_n >= 64 && p.k >= 512 && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
-      p.lda <= (1 << 23) && p.ldb <= (1 << 23) && reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0) {
-    drop_stale_error();
-    f8_tile256_kernel<TA, TB><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
-    return hipGetLastError();
-  }
-  const dim3 grid((unsigned) (((p.n + 127) / 128) * (int64_t) ((p.m + 127) / 128)), (unsigned) parts);
+  const auto tiles = [&](int e) { return ((p.m + e - 1) / e) * (int64_t) ((p.n + e - 1) / e); };
   drop_stale_error();
-  if (p.c_type == BOF_F32) f8_tile_any_kernel<TA, TB, true><<<grid, 256, 0, st>>>(p);
-  else f8_tile_any_kernel<TA, TB, false><<<grid, 256, 0, st>>>(p);
+  if (p.c_type != BOF_F32 && p.m >= 128 && p.n >= 128 && p.k >= 128 && p.lda <= (1 << 26) && p.ldb <= (1 << 26)) {
+    // a slab of 256 x 256 takes a CU about 2200 cycles, one of 128 x 128 about 770
+    const int64_t t256 = (tiles(256) + 255) / 256 * 2200, t128 = (tiles(128) + 255) / 256 * 770;
+    if (parts == 1 && p.m >= 256 && p.n >= 256 && t256 <= t128) start_tiles<TA, TB, 8, 8>(p, 1, st);
+    else start_tiles<TA, TB, 4, 4>(p, parts, st);
+  } else {
+    const dim3 grid((unsigned) tiles(128), (unsigned) parts);
+    if (p.c_type == BOF_F32) f8_tile_any_kernel<TA, TB, true><<<grid, 256, 0, st>>>(p);
+    else f8_tile_any_kernel<TA, TB, false><<<grid, 256, 0, st>>>(p);
+  }
   if (parts > 1) {
     const int64_t wg = ((int64_t) p.m * p.n + 255) / 256;
     f8_join_kernel<<<(unsigned) (wg < 2048 ? wg : 2048), 256, 0, st>>>(p, parts);
