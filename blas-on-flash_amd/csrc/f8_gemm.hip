@@ -525,6 +525,108 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, max(tm * TM, i0 + wi), max(tn * TN, j0 + wj));
 }
 
+// ---- few rows of A -------------------------------------------------------------------
+// Up to 64 rows of A: the bytes of B bound the product.  A workgroup owns 16 NT columns of C and all of k; its waves take the
+// blocks of k in turn, so that every wave streams B (and A, from the caches) straight into registers, UNROLL blocks in
+// flight, and nobody waits for anybody until the waves' sums are added, in their order, through LDS.
+template <int TA, int TB, bool WIDE, int MT, int NT>
+__global__ void __launch_bounds__(512) f8_rows_kernel(F8Product p) {
+  extern __shared__ f32x4 sums[];   // [wave][tile][lane]
+  constexpr int UNROLL = MT == 4 ? 1 : 2;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6;
+  const int l16 = lane & 15, g = lane >> 4, j0 = blockIdx.x * 16 * NT;
+  const int full = p.k >> 7;
+  const uint8_t *a_row[MT], *b_row[NT], *sa_row[MT], *sb_row[NT];
+#pragma unroll
+  for (int x = 0; x < MT; x++) {
+    const int i = min(x * 16 + l16, p.m - 1);
+    a_row[x] = p.a + i * p.lda + g * 16;
+    sa_row[x] = p.sa + (i >> p.a_shift) * p.ldsa;
+  }
+#pragma unroll
+  for (int y = 0; y < NT; y++) {
+    const int j = min(j0 + y * 16 + l16, p.n - 1);
+    b_row[y] = p.b + j * p.ldb + g * 16;
+    sb_row[y] = p.sb + (j >> p.b_shift) * p.ldsb;
+  }
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int x = 0; x < MT * NT; x++) acc[x / NT][x % NT] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Block {
+    u32x4 a[MT][2], b[NT][2];
+    uint8_t sa[MT], sb[NT];
+  };
+  auto fetch = [&](Block &v, int blk) {
+    const int64_t at = (int64_t) blk * 128;
+#pragma unroll
+    for (int y = 0; y < NT; y++) {
+      __builtin_memcpy(&v.b[y][0], b_row[y] + at, 16);
+      __builtin_memcpy(&v.b[y][1], b_row[y] + at + 64, 16);
+      v.sb[y] = sb_row[y][blk];
+    }
+#pragma unroll
+    for (int x = 0; x < MT; x++) {
+      __builtin_memcpy(&v.a[x][0], a_row[x] + at, 16);
+      __builtin_memcpy(&v.a[x][1], a_row[x] + at + 64, 16);
+      v.sa[x] = sa_row[x][blk];
+    }
+  };
+  auto multiply = [&](const Block &v) {
+    Frag<WIDE> fa[MT];
+#pragma unroll
+    for (int x = 0; x < MT; x++) fa[x] = make_frag<TA, WIDE>(v.a[x][0], v.a[x][1], v.sa[x]);
+#pragma unroll
+    for (int y = 0; y < NT; y++) {
+      const Frag<WIDE> fb = make_frag<TB, WIDE>(v.b[y][0], v.b[y][1], v.sb[y]);
+#pragma unroll
+      for (int x = 0; x < MT; x++) acc[x][y] = mma<TA, TB, WIDE>(fb, fa[x], acc[x][y]);
+    }
+  };
+  int blk = wave;
+  for (; blk + (UNROLL - 1) * waves < full; blk += UNROLL * waves) {
+    Block v[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) fetch(v[u], blk + u * waves);
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) multiply(v[u]);
+  }
+  for (; blk < full; blk += waves) {
+    Block v;
+    fetch(v, blk);
+    multiply(v);
+  }
+  if ((p.k & 127) && wave == full % waves) {   // the short block
+    Block v;
+#pragma unroll
+    for (int y = 0; y < NT; y++) {
+      v.b[y][0] = load_chunk(b_row[y] - g * 16, full * 128 + g * 16, p.k);
+      v.b[y][1] = load_chunk(b_row[y] - g * 16, full * 128 + g * 16 + 64, p.k);
+      v.sb[y] = sb_row[y][full];
+    }
+#pragma unroll
+    for (int x = 0; x < MT; x++) {
+      v.a[x][0] = load_chunk(a_row[x] - g * 16, full * 128 + g * 16, p.k);
+      v.a[x][1] = load_chunk(a_row[x] - g * 16, full * 128 + g * 16 + 64, p.k);
+      v.sa[x] = sa_row[x][full];
+    }
+    multiply(v);
+  }
+#pragma unroll
+  for (int x = 0; x < MT * NT; x++) sums[(wave * MT * NT + x) * 64 + lane] = acc[x / NT][x % NT];
+  __syncthreads();
+  for (int at = t; at < MT * NT * 64; at += blockDim.x) {
+    f32x4 v = sums[at];
+    for (int w = 1; w < waves; w++) v += sums[w * MT * NT * 64 + at];
+    const int x = (at >> 6) / NT, y = (at >> 6) % NT;
+    const int i = x * 16 + l16, j = j0 + y * 16 + g * 4;
+    if (i < p.m) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (j + e < p.n) finish(p, i, j + e, v[e]);
+    }
+  }
+}
+
 // C from the parts of the sums, added in their order (no parts: C = beta * C)
 __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
   const int64_t mn = (int64_t) p.m * p.n;
@@ -542,7 +644,7 @@ constexpr int kMaxParts = 32;
 // (the join reads and writes every part again: it pays for itself from about 24 blocks on).
 int wanted_parts(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128), nb = (k + 127) / 128;
-  if (nb < 24) return 1;
+  if (m <= 64 || nb < 24) return 1;
   const int64_t parts = 512 / tiles < nb / 8 ? 512 / tiles : nb / 8;
   return (int) (parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
 }
@@ -559,6 +661,14 @@ void start_tiles(const F8Product &p, int parts, hipStream_t st) {
   else f8_tile_kernel<TA, TB, X, Y, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 
+template <int TA, int TB, int MT, int NT>
+void start_rows(const F8Product &p, hipStream_t st) {
+  const int waves = 8;
+  const unsigned wg = (unsigned) ((p.n + 16 * NT - 1) / (16 * NT)), bytes = waves * MT * NT * 1024;
+  if (p.c_type == BOF_F32) f8_rows_kernel<TA, TB, true, MT, NT><<<wg, 64 * waves, bytes, st>>>(p);
+  else f8_rows_kernel<TA, TB, false, MT, NT><<<wg, 64 * waves, bytes, st>>>(p);
+}
+
 template <int TA, int TB>
 hipError_t launch_product(F8Product p, int parts, hipStream_t st) {
   // parts begin at multiples of four blocks; the short block is the last part's
@@ -568,6 +678,12 @@ hipError_t launch_product(F8Product p, int parts, hipStream_t st) {
   if (parts == 1) p.part = nullptr;
   const auto tiles = [&](int e) { return ((p.m + e - 1) / e) * (int64_t) ((p.n + e - 1) / e); };
   drop_stale_error();
+  if (p.m <= 64 && p.n <= (1 << 26)) {   // (more columns: more threads than a launch holds)
+    if (p.m <= 16) start_rows<TA, TB, 1, 1>(p, st);
+    else if (p.m <= 32) start_rows<TA, TB, 2, 2>(p, st);
+    else start_rows<TA, TB, 4, 2>(p, st);
+    return hipGetLastError();
+  }
   if (p.c_type != BOF_F32 && p.m >= 128 && p.n >= 128 && p.k >= 128 && p.lda <= (1 << 26) && p.ldb <= (1 << 26)) {
     // a slab of 256 x 256 takes a CU about 2200 cycles, one of 128 x 128 about 770
     const int64_t t256 = (tiles(256) + 255) / 256 * 2200, t128 = (tiles(128) + 255) / 256 * 770;
