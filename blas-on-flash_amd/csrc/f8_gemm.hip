@@ -279,16 +279,17 @@ template <int X, int Y>
 __device__ __forceinline__ void store_wave(const F8Product &p, f32x4 (&acc)[X][Y], f32x4 *own, int i, int j, int i_from, int j_from) {
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   constexpr int W = 4 * Y, LANES = 2 * Y;   // chunks in a row, lanes a row
+  constexpr int XP = X < 4 ? X : 4;         // tiles at a time
 #pragma unroll
-  for (int part = 0; part < X / 4; part++) {
+  for (int part = 0; part < X / XP; part++) {
 #pragma unroll
-    for (int x = 0; x < 4; x++)
+    for (int x = 0; x < XP; x++)
 #pragma unroll
-      for (int y = 0; y < Y; y++) own[(x * 16 + l16) * W + ((y * 4 + g) ^ (l16 & 7))] = acc[part * 4 + x][y];
+      for (int y = 0; y < Y; y++) own[(x * 16 + l16) * W + ((y * 4 + g) ^ (l16 & 7))] = acc[part * XP + x][y];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 2
-    for (int it = 0; it < LANES; it++) {
-      const int r = it * (64 / LANES) + lane / LANES, c2 = lane % LANES * 2, row = i + part * 64 + r, col = j + c2 * 4;
+    for (int it = 0; it < XP * 16 * LANES / 64; it++) {
+      const int r = it * (64 / LANES) + lane / LANES, c2 = lane % LANES * 2, row = i + part * XP * 16 + r, col = j + c2 * 4;
       const f32x4 lo = own[r * W + (c2 ^ (r & 7))], hi = own[r * W + ((c2 + 1) ^ (r & 7))];
       if (row < i_from || row >= p.m) continue;
       if (col >= j_from && col + 8 <= p.n) {
@@ -525,6 +526,157 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, max(tm * TM, i0 + wi), max(tn * TN, j0 + wj));
 }
 
+// ---- tiles, wide ---------------------------------------------------------------------
+// A 32-bit C: fragments are widened to bf16 in registers, 16 conversions of 8 cycles for 32 bytes a lane, and multiplied by 4
+// instructions of 16 cycles.  A wave of X x 4 tiles converts X + 4 fragments for 4 X products a block: at X = 8 1536 cycles
+// of conversions beside 2048 of the matrix unit.  To keep both busy a SIMD holds TWO waves: a workgroup of eight owns 32 X rows
+// and 128 columns of C, waves 0-3 work on the even blocks of k, waves 4-7 on the odd ones, each with sums of its own that are
+// added in the end.  The two groups are half a block apart, so that one converts its B fragments while the other multiplies.
+//
+// LDS: three slots of one block (A and B rows of 128 bytes, swizzled as above) and the scale words.  In step t group t & 1
+// begins with block t (slot t % 3) and the other one is in its second half of block t - 1; block t + 1 is fetched into the third
+// slot.  A barrier ends each step.
+template <int X, bool DMA>
+struct WideSlab {
+  static constexpr int A_IMAGE = 256 * X, SLOT = A_IMAGE + 1024;   // chunks of 16 bytes
+  static constexpr int S0 = 3 * SLOT, WORDS = 32 * X + 128, CHUNKS = S0 + WORDS / 2;
+  static constexpr int PIECES = (X + 4) / 2;                       // of 64 rows (8 a wave)
+};
+
+template <int TA, int TB, int X, bool DMA>
+__global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_m, int tiles_n) {
+  using S = WideSlab<X, DMA>;
+  __shared__ u32x4 lds[S::CHUNKS];
+  const F8Product p = part_of(q, blockIdx.y);
+  constexpr int TM = 32 * X, TN = 128, Y = 4;
+  int tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
+  const int i0 = min(tm * TM, p.m - TM), j0 = min(tn * TN, p.n - TN);
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), group = wave >> 2;
+  const int wi = ((wave >> 1) & 1) * 16 * X, wj = (wave & 1) * 64;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int nb = (p.k + 127) >> 7, all = p.k >> 7;
+  const int b0 = blockIdx.y * p.blocks_per_part, full = min(all, b0 + p.blocks_per_part);   // blocks b0 .. full - 1, one at least
+  const bool tail = nb > all && blockIdx.y == gridDim.y - 1;
+  // piece q: rows 64 q + 8 wave + lane / 8 of A and then B
+  const int r8 = lane >> 3, chunk = (DMA ? (lane & 7) ^ r8 : lane & 7) << 4;
+  const uint32_t a_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.lda + chunk, b_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.ldb + chunk;
+  const uint64_t a_step = (uint64_t) p.lda * 64, b_step = (uint64_t) p.ldb * 64;
+  const uint64_t a_org = reinterpret_cast<uint64_t>(p.a + (int64_t) i0 * p.lda), b_org = reinterpret_cast<uint64_t>(p.b + (int64_t) j0 * p.ldb);
+  const uint32_t to = lds_address(lds) + wave * 1024;
+  const int put = (8 * wave + r8) * 8 + ((lane & 7) ^ r8);
+  u32x4 staged[DMA ? 1 : S::PIECES];
+  auto fetch = [&](int blk, int slot) {   // block blk on its way: DMA to LDS, or to registers
+#pragma unroll
+    for (int r = 0; r < S::PIECES; r++) {
+      const bool a = r < X / 2;
+      const uint64_t from = (a ? a_org + r * a_step : b_org + (r - X / 2) * b_step) + (uint64_t) blk * 128;
+      if constexpr (DMA) dma16(a ? a_voff : b_voff, from, to + slot * S::SLOT * 16 + r * 8192);
+      else __builtin_memcpy(&staged[r], reinterpret_cast<const uint8_t *>(from) + (a ? a_voff : b_voff), 16);
+    }
+  };
+  auto land = [&](int slot) {             // ... and there
+    if constexpr (DMA) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+#pragma unroll
+      for (int r = 0; r < S::PIECES; r++) lds[slot * S::SLOT + put + r * 512] = staged[r];
+    }
+  };
+  // scale words: thread t has row t of A and then B
+  uint32_t *const sw = (uint32_t *) (lds + S::S0) + t;
+  const uint8_t *const s_row = t < TM ? p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa : p.sb + (int64_t) ((j0 + min(t - TM, TN - 1)) >> p.b_shift) * p.ldsb;
+  auto put_word = [&](int at, uint32_t w) { if (t < S::WORDS) sw[at] = w; };
+  const int a_lo = (wi + l16) * 8 + (g ^ (l16 & 7)), a_hi = (wi + l16) * 8 + ((g + 4) ^ (l16 & 7));
+  const int b_lo = S::A_IMAGE + (wj + l16) * 8 + (g ^ (l16 & 7)), b_hi = S::A_IMAGE + (wj + l16) * 8 + ((g + 4) ^ (l16 & 7));
+  const uint8_t *const sa = (const uint8_t *) (lds + S::S0) + (wi + l16) * 4, *const sb = (const uint8_t *) (lds + S::S0) + (TM + wj + l16) * 4;
+  f32x4 acc[X][Y];
+#pragma unroll
+  for (int x = 0; x < X * Y; x++) acc[x / Y][x % Y] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Frag<true> fb[Y];
+  auto widen_b = [&](int slot, int byte) {
+#pragma unroll
+    for (int y = 0; y < Y; y++) fb[y] = make_frag<TB, true>(lds[slot * S::SLOT + b_lo + y * 128], lds[slot * S::SLOT + b_hi + y * 128], sb[byte + y * 64]);
+  };
+  auto multiply = [&](int slot, int byte, int x0) {   // X / 2 tiles of A
+#pragma unroll
+    for (int x = x0; x < x0 + X / 2; x++) {
+      const Frag<true> fa = make_frag<TA, true>(lds[slot * S::SLOT + a_lo + x * 128], lds[slot * S::SLOT + a_hi + x * 128], sa[byte + x * 64]);
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int y = 0; y < Y; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[y].q[c], fa.q[c], acc[x][y], 0, 0, 0);
+    }
+  };
+  auto byte_of = [](int kb) { return ((kb & 4) ? S::WORDS * 4 : 0) + (kb & 3); };
+  uint32_t word = 0;
+  int next_slot = 1;
+  // step kb: the next block is fetched; the scales of the next four blocks are fetched in step 0 of four and in LDS by the end of
+  // step 2 (b0 is a multiple of four)
+  auto begin_step = [&](int kb) {
+    if (kb + 1 < full) fetch(kb + 1, next_slot);
+    if ((kb & 3) == 0 && kb + 4 < nb) word = scale_word(s_row, kb + 4, nb);
+  };
+  auto end_step = [&](int kb) {
+    if (kb + 1 < full) land(next_slot);
+    if ((kb & 3) == 2 && kb + 2 < nb) put_word((~kb & 4) ? S::WORDS : 0, word >> scale_shift(kb + 2, nb));
+    next_slot = next_slot == 2 ? 0 : next_slot + 1;
+    __syncthreads();
+  };
+  fetch(b0, 0);
+  put_word((b0 & 4) ? S::WORDS : 0, scale_word(s_row, b0, nb) >> scale_shift(b0, nb));
+  land(0);
+  __syncthreads();
+  if (group == 1) { begin_step(b0); end_step(b0); }
+  int slot = group;
+  int kb = b0 + group;
+  for (; kb < full; kb += 2) {
+    begin_step(kb);
+    widen_b(slot, byte_of(kb));
+    multiply(slot, byte_of(kb), 0);
+    end_step(kb);
+    begin_step(kb + 1);
+    multiply(slot, byte_of(kb), X / 2);
+    end_step(kb + 1);
+    slot = slot == 0 ? 2 : slot - 1;
+  }
+  if (kb == full) end_step(full);   // (the group that ran out first: steps b0 .. full are all of them)
+  if (tail) {   // the short block: through registers, zeros behind k; the first group's
+#pragma unroll 1
+    for (int u = 0; u < S::PIECES; u++) {
+      const int r = 64 * u + 8 * wave + r8;
+      const uint8_t *row = u < X / 2 ? p.a + (int64_t) (i0 + r) * p.lda : p.b + (int64_t) (j0 + r - TM) * p.ldb;
+      lds[put + u * 512] = load_chunk(row, all * 128 + (lane & 7) * 16, p.k);
+    }
+    put_word(0, s_row[all]);
+    __syncthreads();
+    if (group == 0) {
+      widen_b(0, 0);
+      multiply(0, 0, 0);
+      multiply(0, 0, X / 2);
+    }
+    __syncthreads();
+  }
+  // each group stores one half of the rows: it gets the other's sums for them
+  f32x4 *const mine = (f32x4 *) lds + wave * (X / 2 * Y * 64), *const theirs = (f32x4 *) lds + (wave ^ 4) * (X / 2 * Y * 64);
+  f32x4 sum[X / 2][Y];
+#pragma unroll
+  for (int x = 0; x < X / 2; x++)
+#pragma unroll
+    for (int y = 0; y < Y; y++) mine[(x * Y + y) * 64 + lane] = group ? acc[x][y] : acc[x + X / 2][y];
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < X / 2; x++)
+#pragma unroll
+    for (int y = 0; y < Y; y++) {
+      const f32x4 v = theirs[(x * Y + y) * 64 + lane];
+      sum[x][y] = group ? v + acc[x + X / 2][y] : acc[x][y] + v;
+    }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  const int i = i0 + wi + group * X / 2 * 16;
+  store_wave<X / 2, Y>(p, sum, theirs, i, j0 + wj, max(tm * TM, i), max(tn * TN, j0 + wj));
+}
+
 // ---- few rows of A -------------------------------------------------------------------
 // Up to 64 rows of A: the bytes of B bound the product.  A workgroup owns 16 NT columns of C and all of k; its waves take the
 // blocks of k in turn, so that every wave streams B (and A, from the caches) straight into registers, UNROLL blocks in
@@ -661,6 +813,14 @@ void start_tiles(const F8Product &p, int parts, hipStream_t st) {
   else f8_tile_kernel<TA, TB, X, Y, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 
+template <int TA, int TB, int X>
+void start_wide(const F8Product &p, int parts, hipStream_t st) {
+  const int tiles_m = (p.m + 32 * X - 1) / (32 * X), tiles_n = (p.n + 127) / 128;
+  const dim3 grid((unsigned) (tiles_m * tiles_n), (unsigned) parts);
+  if (rows_aligned(p)) f8_wide_kernel<TA, TB, X, true><<<grid, 512, 0, st>>>(p, tiles_m, tiles_n);
+  else f8_wide_kernel<TA, TB, X, false><<<grid, 512, 0, st>>>(p, tiles_m, tiles_n);
+}
+
 template <int TA, int TB, int MT, int NT>
 void start_rows(const F8Product &p, hipStream_t st) {
   const int waves = 8;
@@ -689,6 +849,9 @@ hipError_t launch_product(F8Product p, int parts, hipStream_t st) {
     const int64_t t256 = (tiles(256) + 255) / 256 * 2200, t128 = (tiles(128) + 255) / 256 * 770;
     if (parts == 1 && p.m >= 256 && p.n >= 256 && t256 <= t128) start_tiles<TA, TB, 8, 8>(p, 1, st);
     else start_tiles<TA, TB, 4, 4>(p, parts, st);
+  } else if (p.c_type == BOF_F32 && p.m >= 128 && p.n >= 128 && p.k >= 128 && p.lda <= (1 << 25) && p.ldb <= (1 << 25)) {
+    if (p.m >= 256) start_wide<TA, TB, 8>(p, parts, st);
+    else start_wide<TA, TB, 4>(p, parts, st);
   } else {
     const dim3 grid((unsigned) tiles(128), (unsigned) parts);
     if (p.c_type == BOF_F32) f8_tile_any_kernel<TA, TB, true><<<grid, 256, 0, st>>>(p);
