@@ -51,10 +51,8 @@ struct Frag<true> {
   bf16x8 q[4];
 };
 
-// 2^(code - 127) as a float: code 0 is below the normal floats, 255 is NaN
-__device__ __forceinline__ float scale_value(uint32_t code) {
-  return __uint_as_float(code == 0u ? 0x00400000u : code == 255u ? 0x7fc00000u : code << 23);
-}
+// a scale as the widening instructions take it: they read the exponent field of a float, as E8M0 (0 is 2^-127, 255 is NaN)
+__device__ __forceinline__ float scale_value(uint32_t code) { return __uint_as_float(code << 23); }
 
 template <int T>
 __device__ __forceinline__ bf16x8 widen8(int lo, int hi, float s) {
@@ -228,6 +226,10 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 __device__ __forceinline__ void dma16(uint32_t voff, uint64_t base, uint32_t to) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(voff), "s"(base), "s"(to) : "memory", "m0");
 }
+// one word a lane from `from` to LDS at `to`, which nobody reads: brings the line into the L2
+__device__ __forceinline__ void touch(const uint8_t *from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(from), "s"(to) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // workgroups go round the 8 XCDs; tiles of one XCD are neighbours (each XCD has its own L2), GROUP rows of tiles deep
@@ -337,7 +339,7 @@ template <int X, int Y, bool DMA>
 struct Slab {
   static constexpr int A_IMAGE = 256 * X, B_IMAGE = 256 * Y;       // chunks of 16 bytes in an image
   static constexpr int B0 = 2 * A_IMAGE, S0 = B0 + 2 * B_IMAGE;    // where the B images and the scale words begin
-  static constexpr int WORDS = 32 * (X + Y), CHUNKS = S0 + WORDS / 2;
+  static constexpr int WORDS = 32 * (X + Y), CHUNKS = S0 + WORDS / 2 + 64;
   static constexpr int PIECES = X + Y;                             // of 32 rows (8 a wave)
   u32x4 *lds;
   uint32_t a_voff, b_voff;       // of this thread's row and chunk in a piece
@@ -346,12 +348,14 @@ struct Slab {
   int put;                       // this thread's chunk in a piece (staged)
   int a_lo, a_hi, b_lo, b_hi;    // this lane's chunks in the image, of tile 0
   const uint8_t *sa, *sb;        // this lane's scale bytes of tile 0, block 0 of four
+  const uint8_t *ahead;          // the line this lane touches
+  uint32_t junk;
   u32x4 staged[DMA ? 1 : PIECES];
 };
 
 template <int TA, int TB, int X, int Y, bool DMA, int P>
-__device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64_t a_next, int sc_b, int sc_a, Frag<false> (&fa)[2][X],
-                                     Frag<false> (&fb)[2], f32x4 (&acc)[X][Y]) {
+__device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64_t a_next, uint32_t ahead, int sc_b, int sc_a,
+                                     Frag<false> (&fa)[2][X], Frag<false> (&fb)[2], f32x4 (&acc)[X][Y]) {
   using S = Slab<X, Y, DMA>;
   // piece p: B first, into the other B image; then A, into the image whose fragments are in registers
   auto piece = [&](int q) {
@@ -369,7 +373,7 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
 #pragma unroll
   for (int y = 0; y < Y; y++) {
     if (y == Y - 1) {
-      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -386,6 +390,7 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
       // the pieces: one behind every second MFMA from the start on (4 x 4: behind every one)
       constexpr int D = LAST / S::PIECES >= 2 ? 2 : 1;
       if (at % D == D - 1 && at / D < S::PIECES) piece(at / D);
+      if (DMA && at == D * S::PIECES) touch(s.ahead + ahead, s.junk);
       // the next slab's A fragments: X of them between a quarter and three quarters of the slab
       constexpr int F0 = N / 4, STEP = (LAST - F0 - 2) / X > 4 ? 4 : (LAST - F0 - 2) / X;
       if (at >= F0 && (at - F0) % STEP == 0 && (at - F0) / STEP < X) {
@@ -440,6 +445,12 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   const uint64_t a_org = reinterpret_cast<uint64_t>(p.a + (int64_t) i0 * p.lda), b_org = reinterpret_cast<uint64_t>(p.b + (int64_t) j0 * p.ldb);
   auto a_at = [&](int kb) { return a_org + (uint64_t) min(kb, full - 1) * 128; };   // (behind the last slab: the last one again)
   auto b_at = [&](int kb) { return b_org + (uint64_t) min(kb, full - 1) * 128; };
+  auto ahead_at = [&](int kb) { return (uint32_t) min(kb + 4, full - 1) * 128u; };
+  {
+    const int r = wave * 16 + l16, half = (lane & 32) * 2;
+    s.ahead = (lane & 16 ? p.b + (int64_t) (j0 + (tm & 3) * (TN / 4) + r % (TN / 4)) * p.ldb : p.a + (int64_t) (i0 + (tn & 3) * (TM / 4) + r % (TM / 4)) * p.lda) + half;
+    s.junk = lds_address(lds) + (S::S0 + S::WORDS / 2) * 16 + wave * 256;
+  }
   f32x4 acc[X][Y];
 #pragma unroll
   for (int x = 0; x < X * Y; x++) acc[x / Y][x % Y] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -492,10 +503,10 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   int kb = b0;
   for (; kb + 2 <= full; kb += 2) {
     words(kb);
-    slab<TA, TB, X, Y, DMA, 0>(s, DMA ? b_at(kb + 1) : b_at(kb + 2), DMA ? a_at(kb + 2) : a_at(kb + 3), byte_of(kb), byte_of(kb + 1), fa, fb, acc);
-    slab<TA, TB, X, Y, DMA, 1>(s, DMA ? b_at(kb + 2) : b_at(kb + 3), DMA ? a_at(kb + 3) : a_at(kb + 4), byte_of(kb + 1), byte_of(kb + 2), fa, fb, acc);
+    slab<TA, TB, X, Y, DMA, 0>(s, DMA ? b_at(kb + 1) : b_at(kb + 2), DMA ? a_at(kb + 2) : a_at(kb + 3), ahead_at(kb), byte_of(kb), byte_of(kb + 1), fa, fb, acc);
+    slab<TA, TB, X, Y, DMA, 1>(s, DMA ? b_at(kb + 2) : b_at(kb + 3), DMA ? a_at(kb + 3) : a_at(kb + 4), ahead_at(kb + 1), byte_of(kb + 1), byte_of(kb + 2), fa, fb, acc);
   }
-  if (kb < full) slab<TA, TB, X, Y, DMA, 0>(s, b_at(kb), a_at(kb), byte_of(kb), byte_of(kb), fa, fb, acc);
+  if (kb < full) slab<TA, TB, X, Y, DMA, 0>(s, b_at(kb), a_at(kb), ahead_at(kb), byte_of(kb), byte_of(kb), fa, fb, acc);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   if (tail) {   // the short block: through registers, zeros behind k
@@ -527,16 +538,15 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
 }
 
 // ---- tiles, wide ---------------------------------------------------------------------
-// A 32-bit C: fragments are widened to bf16 in registers, 16 conversions of 8 cycles for 32 bytes a lane, and multiplied by 4
-// instructions of 16 cycles.  A wave of X x 4 tiles converts X + 4 fragments for 4 X products a block: at X = 8 1536 cycles
-// of conversions beside 2048 of the matrix unit.  To keep both busy a SIMD holds TWO waves: a workgroup of eight owns 32 X rows
-// and 128 columns of C, waves 0-3 work on the even blocks of k, waves 4-7 on the odd ones, each with sums of its own that are
-// added in the end.  The two groups are half a block apart, so that one converts its B fragments while the other multiplies.
+// A 32-bit C: fragments are widened to bf16 in registers, 8 conversions for 16 bytes a lane, and multiplied by 2
+// instructions of 16 cycles.  A SIMD holds TWO waves, so that one converts while the other multiplies: a workgroup of eight
+// owns 32 X rows and 128 columns of C, waves 0-3 work on the first half of every block of k, waves 4-7 on the second, each
+// with sums of its own that are added in the end.
 //
-// LDS: three slots of one block (A and B rows of 128 bytes, swizzled as above) and the scale words.  In step t group t & 1
-// begins with block t (slot t % 3) and the other one is in its second half of block t - 1; block t + 1 is fetched into the third
-// slot.  A barrier ends each step.
-template <int X, bool DMA>
+// LDS: three slots of one block (A and B rows of 128 bytes, swizzled as above) and the scale words.  Step t multiplies block t
+// out of registers, reads block t + 1 into them -- every fragment as soon as its predecessor is widened -- and fetches block
+// t + 3 into the slot that block t has left: a piece has two steps to land, a fragment one.  A barrier ends each step.
+template <int X>
 struct WideSlab {
   static constexpr int A_IMAGE = 256 * X, SLOT = A_IMAGE + 1024;   // chunks of 16 bytes
   static constexpr int S0 = 3 * SLOT, WORDS = 32 * X + 128, CHUNKS = S0 + WORDS / 2;
@@ -545,7 +555,7 @@ struct WideSlab {
 
 template <int TA, int TB, int X, bool DMA>
 __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_m, int tiles_n) {
-  using S = WideSlab<X, DMA>;
+  using S = WideSlab<X>;
   __shared__ u32x4 lds[S::CHUNKS];
   const F8Product p = part_of(q, blockIdx.y);
   constexpr int TM = 32 * X, TN = 128, Y = 4;
@@ -558,7 +568,7 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   const int nb = (p.k + 127) >> 7, all = p.k >> 7;
   const int b0 = blockIdx.y * p.blocks_per_part, full = min(all, b0 + p.blocks_per_part);   // blocks b0 .. full - 1, one at least
   const bool tail = nb > all && blockIdx.y == gridDim.y - 1;
-  // piece q: rows 64 q + 8 wave + lane / 8 of A and then B
+  // piece r: rows 64 r + 8 wave + lane / 8 of A and then B
   const int r8 = lane >> 3, chunk = (DMA ? (lane & 7) ^ r8 : lane & 7) << 4;
   const uint32_t a_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.lda + chunk, b_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.ldb + chunk;
   const uint64_t a_step = (uint64_t) p.lda * 64, b_step = (uint64_t) p.ldb * 64;
@@ -566,19 +576,17 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   const uint32_t to = lds_address(lds) + wave * 1024;
   const int put = (8 * wave + r8) * 8 + ((lane & 7) ^ r8);
   u32x4 staged[DMA ? 1 : S::PIECES];
-  auto fetch = [&](int blk, int slot) {   // block blk on its way: DMA to LDS, or to registers
+  auto fetch = [&](int blk, int slot) {   // a block (behind the last one: the last one again) on its way: DMA to LDS, or to registers
 #pragma unroll
     for (int r = 0; r < S::PIECES; r++) {
       const bool a = r < X / 2;
-      const uint64_t from = (a ? a_org + r * a_step : b_org + (r - X / 2) * b_step) + (uint64_t) blk * 128;
+      const uint64_t from = (a ? a_org + r * a_step : b_org + (r - X / 2) * b_step) + (uint64_t) min(blk, full - 1) * 128;
       if constexpr (DMA) dma16(a ? a_voff : b_voff, from, to + slot * S::SLOT * 16 + r * 8192);
       else __builtin_memcpy(&staged[r], reinterpret_cast<const uint8_t *>(from) + (a ? a_voff : b_voff), 16);
     }
   };
-  auto land = [&](int slot) {             // ... and there
-    if constexpr (DMA) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    } else {
+  auto land = [&](int slot) {             // ... and there (staged)
+    if constexpr (!DMA) {
 #pragma unroll
       for (int r = 0; r < S::PIECES; r++) lds[slot * S::SLOT + put + r * 512] = staged[r];
     }
@@ -587,61 +595,67 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   uint32_t *const sw = (uint32_t *) (lds + S::S0) + t;
   const uint8_t *const s_row = t < TM ? p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa : p.sb + (int64_t) ((j0 + min(t - TM, TN - 1)) >> p.b_shift) * p.ldsb;
   auto put_word = [&](int at, uint32_t w) { if (t < S::WORDS) sw[at] = w; };
-  const int a_lo = (wi + l16) * 8 + (g ^ (l16 & 7)), a_hi = (wi + l16) * 8 + ((g + 4) ^ (l16 & 7));
-  const int b_lo = S::A_IMAGE + (wj + l16) * 8 + (g ^ (l16 & 7)), b_hi = S::A_IMAGE + (wj + l16) * 8 + ((g + 4) ^ (l16 & 7));
+  // this lane's chunk in an image, of tile 0: its half of the block
+  const int a_at = (wi + l16) * 8 + ((4 * group + g) ^ (l16 & 7)), b_at = S::A_IMAGE + (wj + l16) * 8 + ((4 * group + g) ^ (l16 & 7));
   const uint8_t *const sa = (const uint8_t *) (lds + S::S0) + (wi + l16) * 4, *const sb = (const uint8_t *) (lds + S::S0) + (TM + wj + l16) * 4;
+  auto byte_of = [](int kb) { return ((kb & 4) ? S::WORDS * 4 : 0) + (kb & 3); };
   f32x4 acc[X][Y];
 #pragma unroll
   for (int x = 0; x < X * Y; x++) acc[x / Y][x % Y] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Frag<true> fb[Y];
-  auto widen_b = [&](int slot, int byte) {
+  u32x4 ra[X], rb[Y];   // the block that is multiplied next, as it lies in memory
+  bf16x8 b[Y][2];
+  // one block out of registers; its successor is read from `next`
+  auto multiply = [&](int next, int byte) {
+    const u32x4 *const img = lds + next * S::SLOT;
 #pragma unroll
-    for (int y = 0; y < Y; y++) fb[y] = make_frag<TB, true>(lds[slot * S::SLOT + b_lo + y * 128], lds[slot * S::SLOT + b_hi + y * 128], sb[byte + y * 64]);
-  };
-  auto multiply = [&](int slot, int byte, int x0) {   // X / 2 tiles of A
+    for (int y = 0; y < Y; y++) {
+      const float sc = scale_value(sb[byte + y * 64]);
+      b[y][0] = widen8<TB>((int) rb[y][0], (int) rb[y][1], sc);
+      b[y][1] = widen8<TB>((int) rb[y][2], (int) rb[y][3], sc);
+      rb[y] = img[b_at + y * 128];
+    }
 #pragma unroll
-    for (int x = x0; x < x0 + X / 2; x++) {
-      const Frag<true> fa = make_frag<TA, true>(lds[slot * S::SLOT + a_lo + x * 128], lds[slot * S::SLOT + a_hi + x * 128], sa[byte + x * 64]);
+    for (int x = 0; x < X; x++) {
+      const float sc = scale_value(sa[byte + x * 64]);
+      const bf16x8 a0 = widen8<TA>((int) ra[x][0], (int) ra[x][1], sc), a1 = widen8<TA>((int) ra[x][2], (int) ra[x][3], sc);
+      ra[x] = img[a_at + x * 128];
 #pragma unroll
-      for (int c = 0; c < 4; c++)
+      for (int y = 0; y < Y; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y][0], a0, acc[x][y], 0, 0, 0);
 #pragma unroll
-        for (int y = 0; y < Y; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[y].q[c], fa.q[c], acc[x][y], 0, 0, 0);
+      for (int y = 0; y < Y; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[y][1], a1, acc[x][y], 0, 0, 0);
     }
   };
-  auto byte_of = [](int kb) { return ((kb & 4) ? S::WORDS * 4 : 0) + (kb & 3); };
-  uint32_t word = 0;
-  int next_slot = 1;
-  // step kb: the next block is fetched; the scales of the next four blocks are fetched in step 0 of four and in LDS by the end of
-  // step 2 (b0 is a multiple of four)
-  auto begin_step = [&](int kb) {
-    if (kb + 1 < full) fetch(kb + 1, next_slot);
-    if ((kb & 3) == 0 && kb + 4 < nb) word = scale_word(s_row, kb + 4, nb);
-  };
-  auto end_step = [&](int kb) {
-    if (kb + 1 < full) land(next_slot);
-    if ((kb & 3) == 2 && kb + 2 < nb) put_word((~kb & 4) ? S::WORDS : 0, word >> scale_shift(kb + 2, nb));
-    next_slot = next_slot == 2 ? 0 : next_slot + 1;
+  auto read_first = [&](int slot) {
+#pragma unroll
+    for (int x = 0; x < X; x++) ra[x] = lds[slot * S::SLOT + a_at + x * 128];
+#pragma unroll
+    for (int y = 0; y < Y; y++) rb[y] = lds[slot * S::SLOT + b_at + y * 128];
     __syncthreads();
   };
-  fetch(b0, 0);
+  fetch(b0, 0); land(0);
+  fetch(b0 + 1, 1); land(1);
+  fetch(b0 + 2, 2);
   put_word((b0 & 4) ? S::WORDS : 0, scale_word(s_row, b0, nb) >> scale_shift(b0, nb));
-  land(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (group == 1) { begin_step(b0); end_step(b0); }
-  int slot = group;
-  int kb = b0 + group;
-  for (; kb < full; kb += 2) {
-    begin_step(kb);
-    widen_b(slot, byte_of(kb));
-    multiply(slot, byte_of(kb), 0);
-    end_step(kb);
-    begin_step(kb + 1);
-    multiply(slot, byte_of(kb), X / 2);
-    end_step(kb + 1);
-    slot = slot == 0 ? 2 : slot - 1;
+  read_first(0);
+  uint32_t word = 0;
+  int slot = 0;   // of block kb
+  for (int kb = b0; kb < full; kb++) {
+    // the scales of the next four blocks (b0 is a multiple of four): fetched in step 0 of four, in LDS by the end of step 2
+    if ((kb & 3) == 0 && kb + 4 < nb) word = scale_word(s_row, kb + 4, nb);
+    const int next = slot == 2 ? 0 : slot + 1;
+    if constexpr (!DMA) land(next == 2 ? 0 : next + 1);   // (block kb + 2, fetched in the step before)
+    fetch(kb + 3, slot);
+    multiply(next, byte_of(kb));
+    if ((kb & 3) == 2 && kb + 2 < nb) put_word((~kb & 4) ? S::WORDS : 0, word >> scale_shift(kb + 2, nb));
+    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(S::PIECES) : "memory");   // block kb + 2 has landed
+    __syncthreads();
+    slot = next;
   }
-  if (kb == full) end_step(full);   // (the group that ran out first: steps b0 .. full are all of them)
-  if (tail) {   // the short block: through registers, zeros behind k; the first group's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tail) {   // the short block: through registers, zeros behind k
 #pragma unroll 1
     for (int u = 0; u < S::PIECES; u++) {
       const int r = 64 * u + 8 * wave + r8;
@@ -650,11 +664,8 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
     }
     put_word(0, s_row[all]);
     __syncthreads();
-    if (group == 0) {
-      widen_b(0, 0);
-      multiply(0, 0, 0);
-      multiply(0, 0, X / 2);
-    }
+    read_first(0);
+    multiply(0, 0);
     __syncthreads();
   }
   // each group stores one half of the rows: it gets the other's sums for them
