@@ -210,7 +210,11 @@ __global__ void __launch_bounds__(256) f8_tile_any_kernel(F8Product p) {
 // The A fragments of a slab are read into registers during the slab BEFORE (twice X x 8 registers), the B fragments one tile
 // ahead.  The barrier of a slab stands in front of its last row of tiles: by then every wave has read all it wants from this
 // slab's B image and the next slab's A image, and the pieces of the next B and the next but one A image, issued at the slab's
-// start, have landed.
+// start, have landed.  That is time enough from the L2, not from memory, and a CU has only so many misses in flight: so with
+// 8 x 8 every lane also touches one line of the slab but three or four, a quarter of the tile's rows a workgroup -- those of an
+// XCD that share the rows touch the other quarters (8192 cubed, zeros for data: 410 us without, 329 us with).
+//
+// Bound by the card's power at 8192 cubed: 329 us (3.3 PFLOP/s) on zeros, 385 us (2.86) on random bytes.
 //
 // Scales: a thread fetches the word with four blocks' scales of its rows, once in four slabs, into LDS (twice); a fragment's
 // scale byte is read from there along with it.  No vector instruction is left in a slab but a few for the whole of it.
@@ -341,6 +345,7 @@ struct Slab {
   static constexpr int B0 = 2 * A_IMAGE, S0 = B0 + 2 * B_IMAGE;    // where the B images and the scale words begin
   static constexpr int WORDS = 32 * (X + Y), CHUNKS = S0 + WORDS / 2 + 64;
   static constexpr int PIECES = X + Y;                             // of 32 rows (8 a wave)
+  static constexpr bool TOUCH = DMA && X == 8;
   u32x4 *lds;
   uint32_t a_voff, b_voff;       // of this thread's row and chunk in a piece
   uint64_t a_step, b_step;       // bytes from piece to piece
@@ -373,7 +378,7 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
 #pragma unroll
   for (int y = 0; y < Y; y++) {
     if (y == Y - 1) {
-      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(1)" ::: "memory");
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(S::TOUCH ? 1 : 0) : "memory");
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -387,10 +392,12 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
         fb[(y + 1) & 1].q = both(s.lds[s.b_lo + from], s.lds[s.b_hi + from]);
         fb[(y + 1) & 1].s = s.sb[(y < Y - 1 ? sc_b : sc_a) + (y < Y - 1 ? y + 1 : 0) * 64];
       }
-      // the pieces: one behind every second MFMA from the start on (4 x 4: behind every one)
-      constexpr int D = LAST / S::PIECES >= 2 ? 2 : 1;
-      if (at % D == D - 1 && at / D < S::PIECES) piece(at / D);
-      if (DMA && at == D * S::PIECES) touch(s.ahead + ahead, s.junk);
+      // the pieces: behind two MFMAs of three from the start on (4 x 4: behind every one), then the touch, which is waited for
+      // at the barrier of the next slab.  (One piece for every MFMA is more than the texture unit takes, one for every second or
+      // third gives them less time to land: 8192 cubed 329 us, 349, 334 and 365 for zeros.)
+      const int q = X == 8 ? at / 3 * 2 + at % 3 : at;
+      if ((X < 8 || at % 3 != 2) && q < S::PIECES) piece(q);
+      if (S::TOUCH && at == S::PIECES / 2 * 3) touch(s.ahead + ahead, s.junk);
       // the next slab's A fragments: X of them between a quarter and three quarters of the slab
       constexpr int F0 = N / 4, STEP = (LAST - F0 - 2) / X > 4 ? 4 : (LAST - F0 - 2) / X;
       if (at >= F0 && (at - F0) % STEP == 0 && (at - F0) / STEP < X) {
@@ -793,6 +800,21 @@ __global__ void __launch_bounds__(512) f8_rows_kernel(F8Product p) {
 // C from the parts of the sums, added in their order (no parts: C = beta * C)
 __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
   const int64_t mn = (int64_t) p.m * p.n;
+  if (p.n % 8 == 0) {   // eight neighbours a thread
+    for (int64_t at = ((int64_t) blockIdx.x * 256 + threadIdx.x) * 8; at < mn; at += (int64_t) gridDim.x * 2048) {
+      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll 4
+      for (int z = 0; z < parts; z++) {
+        lo += *(const f32x4 *) (p.part + z * mn + at);
+        hi += *(const f32x4 *) (p.part + z * mn + at + 4);
+      }
+      const int64_t c = at / p.n * p.ldc + at % p.n;
+      if (p.c_type == BOF_BF16) finish_eight<BOF_BF16>(p, c, lo, hi);
+      else if (p.c_type == BOF_F16) finish_eight<BOF_F16>(p, c, lo, hi);
+      else finish_eight<BOF_F32>(p, c, lo, hi);
+    }
+    return;
+  }
   for (int64_t at = (int64_t) blockIdx.x * 256 + threadIdx.x; at < mn; at += (int64_t) gridDim.x * 256) {
     float sum = 0.f;
     for (int z = 0; z < parts; z++) sum += p.part[z * mn + at];
