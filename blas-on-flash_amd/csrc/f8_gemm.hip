@@ -17,6 +17,9 @@
 // 2.4e-9 relative on 32 products) at half the rate.
 #include "f8_common.h"
 
+#include <type_traits>
+#include <utility>
+
 namespace bof {
 
 namespace {
@@ -119,24 +122,26 @@ __device__ __forceinline__ void finish(const F8Product &p, int64_t i, int64_t j,
 }
 
 // ---- tiles of any shape and alignment -----------------------------------------------
-// 16 bytes of a row from byte k0 on, zeros from byte k on.  Only a row's last chunk is short: it is read as the row's
-// last 16 bytes and shifted (or byte by byte, in rows shorter than that).
+// 16 bytes of a row from byte k0 on, zeros from byte k on.  A chunk that ends behind the row is read as the row's last 16 bytes
+// and shifted: no branch, so that several may be in flight.
+__device__ __forceinline__ u32x4 load_chunk_of_16(const uint8_t *row, int k0, int k) {   // k >= 16
+  const int at = min(k0, k - 16), over = k0 - at;
+  unsigned __int128 w;
+  __builtin_memcpy(&w, row + at, 16);
+  w = over < 16 ? w >> (8 * over) : 0;
+  u32x4 v;
+  __builtin_memcpy(&v, &w, 16);
+  return v;
+}
 __device__ __forceinline__ u32x4 load_chunk(const uint8_t *row, int k0, int k) {
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (k0 + 16 <= k) {
-    __builtin_memcpy(&v, row + k0, 16);
-  } else if (k0 < k) {
-    if (k >= 16) {
-      unsigned __int128 w;
-      __builtin_memcpy(&w, row + k - 16, 16);
-      w >>= 8 * (k0 + 16 - k);
-      __builtin_memcpy(&v, &w, 16);
-    } else {
-      uint8_t tmp[16];
+  if (k >= 16) return load_chunk_of_16(row, k0, k);
+  u32x4 v;
 #pragma unroll
-      for (int i = 0; i < 16; i++) tmp[i] = k0 + i < k ? row[k0 + i] : 0;
-      __builtin_memcpy(&v, tmp, 16);
-    }
+  for (int e = 0; e < 4; e++) {
+    v[e] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (k0 + 4 * e + i < k) v[e] |= (uint32_t) row[k0 + 4 * e + i] << (8 * i);
   }
   return v;
 }
@@ -153,11 +158,10 @@ __global__ void __launch_bounds__(256) f8_tile_any_kernel(F8Product p) {
   const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
   const int l16 = lane & 15, g = lane >> 4;
   const int nb = (p.k + 127) >> 7;
-  const int b0 = blockIdx.y * p.blocks_per_part, b1 = blockIdx.y == gridDim.y - 1 ? nb : b0 + p.blocks_per_part;
   f32x4 acc[4][4];
 #pragma unroll
   for (int x = 0; x < 16; x++) acc[x >> 2][x & 3] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int blk = b0; blk < b1; blk++) {
+  for (int blk = 0; blk < nb; blk++) {
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       const int at = t + 256 * u, r = at >> 3, c = at & 7;
@@ -189,35 +193,31 @@ __global__ void __launch_bounds__(256) f8_tile_any_kernel(F8Product p) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int i = i0 + wi + x * 16 + l16, j = j0 + wj + y * 16 + g * 4 + e;
-        if (i < p.m && j < p.n) {
-          if (p.part) p.part[((int64_t) blockIdx.y * p.m + i) * p.n + j] = acc[x][y][e];
-          else finish(p, i, j, acc[x][y][e]);
-        }
+        if (i < p.m && j < p.n) finish(p, i, j, acc[x][y][e]);
       }
 }
 
 // ---- tiles ---------------------------------------------------------------------------
 // Four waves, X x Y tiles of 16 x 16 each, 2 x 2 waves: a workgroup owns 32 X rows and 32 Y columns of C.  8 x 8 (256 x 256):
 // one wave on each SIMD, 64 accumulators of four floats = 256 registers (the accumulator half of the file), the other half
-// holds the fragments.  4 x 4 (128 x 128): two workgroups a CU, for outputs with few tiles.
+// holds the fragments.
 //
 // A slab is one block of k: rows of 128 bytes; both operands lie in LDS twice.  DMA: rows reach LDS without touching
 // registers -- one global_load_lds_dwordx4 moves 8 rows, lane l fetching chunk (l & 7) ^ (l >> 3) of row l >> 3, so that the
 // image is [row][chunk ^ (row & 7)] and a fragment read (16 rows x 16 bytes) meets every bank once.  It needs rows aligned to
-// 16 bytes; for others (DMA = false) a thread loads its 16-byte chunks of the same rows, unaligned, and writes them to the
+// four bytes; for others (DMA = false) a thread loads its 16-byte chunks of the same rows, unaligned, and writes them to the
 // same places one slab later.  Per slab and wave of 8 x 8: 64 MFMAs of 32 cycles, 32 ds_read_b128, 16 pieces.
 //
 // The A fragments of a slab are read into registers during the slab BEFORE (twice X x 8 registers), the B fragments one tile
 // ahead.  The barrier of a slab stands in front of its last row of tiles: by then every wave has read all it wants from this
 // slab's B image and the next slab's A image, and the pieces of the next B and the next but one A image, issued at the slab's
-// start, have landed.  That is time enough from the L2, not from memory, and a CU has only so many misses in flight: so with
-// 8 x 8 every lane also touches one line of the slab but three or four, a quarter of the tile's rows a workgroup -- those of an
+// start, have landed.  That is time enough from the L2, not from memory, and a CU has only so many misses in flight: so
+// every lane also touches one line of the slab but three or four, a quarter of the tile's rows a workgroup -- those of an
 // XCD that share the rows touch the other quarters (8192 cubed, zeros for data: 410 us without, 329 us with).
 //
 // Bound by the card's power at 8192 cubed: 329 us (3.3 PFLOP/s) on zeros, 385 us (2.86) on random bytes.
 //
-// Scales: a thread fetches the word with four blocks' scales of its rows, once in four slabs, into LDS (twice); a fragment's
-// scale byte is read from there along with it.  No vector instruction is left in a slab but a few for the whole of it.
+// A fragment's scale byte is read from LDS along with it.  No vector instruction is left in a slab but a few for the whole of it.
 //
 // A tile at the lower or right edge starts earlier (at m - 32 X, n - 32 Y), so that every row it fetches exists; what lies in
 // the tile before is not stored again.
@@ -245,20 +245,23 @@ __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int g
   tn = bid % per / deep;
 }
 
-// The four scale bytes of blocks b .. b + 3 of a row of nb > b as one word, read inside the row: the word that is read begins
-// up to three bytes early, scale_shift bits of it are left out (rows of fewer than four bytes are read byte by byte).
-__device__ __forceinline__ uint32_t scale_word(const uint8_t *row, int b, int nb) {
-  uint32_t w;
-  if (nb >= 4) {
-    __builtin_memcpy(&w, row + min(b, nb - 4), 4);
-  } else {
-    w = row[0];
-    if (nb > 1) w |= (uint32_t) row[1] << 8;
-    if (nb > 2) w |= (uint32_t) row[2] << 16;
-  }
-  return w;
+// Scales in LDS: for every row of a tile the bytes of 32 blocks, in two halves of 16, 20 bytes from row to row (no bank twice).
+// Both halves are filled in front of the loop over k; later on, when the loop enters a half, the other one is filled with the
+// bytes behind it.  (That waits for all that is in flight, once in 16 blocks: rows of up to 4096 never do.)
+constexpr int scale_chunks(int rows) { return (rows * 40 + 15) / 16; }   // of 16 bytes, both halves
+__device__ __forceinline__ int scale_byte(int kb, int rows) { return ((kb >> 4) & 1) * rows * 20 + (kb & 15); }
+// (in the loop: rows are longer than 16 there.  The wait is one that the compiler sees: else it puts its own, for a register that
+// may still be loading, in front of every step's reads, and with it waits for the pieces in flight)
+__device__ __forceinline__ u32x4 next_scales(const uint8_t *row, int b, int nb) {
+  const u32x4 v = load_chunk_of_16(row, b, nb);
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+  return v;
 }
-__device__ __forceinline__ int scale_shift(int b, int nb) { return 8 * max(0, b - max(nb - 4, 0)); }
+__device__ __forceinline__ void put_scales(uint8_t *half, int row, u32x4 v) {
+  uint32_t *to = (uint32_t *) (half + row * 20);
+#pragma unroll
+  for (int e = 0; e < 4; e++) to[e] = v[e];
+}
 
 __device__ __forceinline__ i32x8 both(u32x4 lo, u32x4 hi) {
   return i32x8{(int) lo[0], (int) lo[1], (int) lo[2], (int) lo[3], (int) hi[0], (int) hi[1], (int) hi[2], (int) hi[3]};
@@ -286,17 +289,18 @@ __device__ __forceinline__ void store_wave(const F8Product &p, f32x4 (&acc)[X][Y
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   constexpr int W = 4 * Y, LANES = 2 * Y;   // chunks in a row, lanes a row
   constexpr int XP = X < 4 ? X : 4;         // tiles at a time
+  constexpr int SWZ = W % 8 ? 3 : 7;
 #pragma unroll
   for (int part = 0; part < X / XP; part++) {
 #pragma unroll
     for (int x = 0; x < XP; x++)
 #pragma unroll
-      for (int y = 0; y < Y; y++) own[(x * 16 + l16) * W + ((y * 4 + g) ^ (l16 & 7))] = acc[part * XP + x][y];
+      for (int y = 0; y < Y; y++) own[(x * 16 + l16) * W + ((y * 4 + g) ^ (l16 & SWZ))] = acc[part * XP + x][y];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 2
     for (int it = 0; it < XP * 16 * LANES / 64; it++) {
-      const int r = it * (64 / LANES) + lane / LANES, c2 = lane % LANES * 2, row = i + part * XP * 16 + r, col = j + c2 * 4;
-      const f32x4 lo = own[r * W + (c2 ^ (r & 7))], hi = own[r * W + ((c2 + 1) ^ (r & 7))];
+      const int r = (it * 64 + lane) / LANES, c2 = (it * 64 + lane) % LANES * 2, row = i + part * XP * 16 + r, col = j + c2 * 4;
+      const f32x4 lo = own[r * W + (c2 ^ (r & SWZ))], hi = own[r * W + ((c2 + 1) ^ (r & SWZ))];
       if (row < i_from || row >= p.m) continue;
       if (col >= j_from && col + 8 <= p.n) {
         const int64_t at = (int64_t) row * p.ldc + col;
@@ -313,17 +317,13 @@ __device__ __forceinline__ void store_wave(const F8Product &p, f32x4 (&acc)[X][Y
   }
 }
 
-// The slab's product, its accumulators pinned (left to itself the compiler moves them through both halves of the register
-// file: 200 copies a slab): to the accumulator half where they are 256, else to the other.  Hazards: the same accumulator
-// comes round after 16 of these at least, the fragments come from LDS; whoever reads acc afterwards calls settle() first.
-template <int TA, int TB, bool AGPR>
+// The slab's product, its accumulators pinned to the accumulator half of the register file (left to itself the compiler moves
+// them through both: 200 copies a slab).  Hazards: the same accumulator comes round after 16 of these at least, the
+// fragments come from LDS; whoever reads acc afterwards calls settle() first.
+template <int TA, int TB>
 __device__ __forceinline__ void mma_pinned(const Frag<false> &b, const Frag<false> &a, f32x4 &acc) {
-  if constexpr (AGPR)
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
-                 : "+a"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
-  else
-    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
-                 : "+v"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
+               : "+a"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
 }
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
@@ -342,17 +342,17 @@ __device__ __forceinline__ F8Product part_of(F8Product p, int z) {
 template <int X, int Y, bool DMA>
 struct Slab {
   static constexpr int A_IMAGE = 256 * X, B_IMAGE = 256 * Y;       // chunks of 16 bytes in an image
-  static constexpr int B0 = 2 * A_IMAGE, S0 = B0 + 2 * B_IMAGE;    // where the B images and the scale words begin
-  static constexpr int WORDS = 32 * (X + Y), CHUNKS = S0 + WORDS / 2 + 64;
+  static constexpr int B0 = 2 * A_IMAGE, S0 = B0 + 2 * B_IMAGE;    // where the B images and the scales begin
+  static constexpr int J0 = S0 + scale_chunks(32 * (X + Y)), CHUNKS = J0 + 64;   // scales, and where touches go
   static constexpr int PIECES = X + Y;                             // of 32 rows (8 a wave)
-  static constexpr bool TOUCH = DMA && X == 8;
+  static constexpr bool TOUCH = DMA;
   u32x4 *lds;
   uint32_t a_voff, b_voff;       // of this thread's row and chunk in a piece
   uint64_t a_step, b_step;       // bytes from piece to piece
   uint32_t a_to, b_to;           // LDS addresses of this wave's pieces in image 0 (DMA)
   int put;                       // this thread's chunk in a piece (staged)
   int a_lo, a_hi, b_lo, b_hi;    // this lane's chunks in the image, of tile 0
-  const uint8_t *sa, *sb;        // this lane's scale bytes of tile 0, block 0 of four
+  const uint8_t *sa, *sb;        // this lane's scale bytes of tile 0
   const uint8_t *ahead;          // the line this lane touches
   uint32_t junk;
   u32x4 staged[DMA ? 1 : PIECES];
@@ -386,24 +386,24 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
 #pragma unroll
     for (int x = 0; x < X; x++) {
       const int at = y * X + x;
-      mma_pinned<TA, TB, X * Y == 64>(fb[y & 1], fa[P][x], acc[x][y]);
+      mma_pinned<TA, TB>(fb[y & 1], fa[P][x], acc[x][y]);
       if (x == 1) {   // the next B tile: of this slab, or the next one's first
         const int from = (y < Y - 1 ? P : P ^ 1) * S::B_IMAGE + (y < Y - 1 ? y + 1 : 0) * 128;
         fb[(y + 1) & 1].q = both(s.lds[s.b_lo + from], s.lds[s.b_hi + from]);
-        fb[(y + 1) & 1].s = s.sb[(y < Y - 1 ? sc_b : sc_a) + (y < Y - 1 ? y + 1 : 0) * 64];
+        fb[(y + 1) & 1].s = s.sb[(y < Y - 1 ? sc_b : sc_a) + (y < Y - 1 ? y + 1 : 0) * 320];
       }
-      // the pieces: behind two MFMAs of three from the start on (4 x 4: behind every one), then the touch, which is waited for
+      // the pieces: behind two MFMAs of three from the start on, then the touch, which is waited for
       // at the barrier of the next slab.  (One piece for every MFMA is more than the texture unit takes, one for every second or
       // third gives them less time to land: 8192 cubed 329 us, 349, 334 and 365 for zeros.)
-      const int q = X == 8 ? at / 3 * 2 + at % 3 : at;
-      if ((X < 8 || at % 3 != 2) && q < S::PIECES) piece(q);
+      const int q = at / 3 * 2 + at % 3;
+      if (at % 3 != 2 && q < S::PIECES) piece(q);
       if (S::TOUCH && at == S::PIECES / 2 * 3) touch(s.ahead + ahead, s.junk);
       // the next slab's A fragments: X of them between a quarter and three quarters of the slab
       constexpr int F0 = N / 4, STEP = (LAST - F0 - 2) / X > 4 ? 4 : (LAST - F0 - 2) / X;
       if (at >= F0 && (at - F0) % STEP == 0 && (at - F0) / STEP < X) {
         const int f = (at - F0) / STEP, from = (P ^ 1) * S::A_IMAGE + f * 128;
         fa[P ^ 1][f].q = both(s.lds[s.a_lo + from], s.lds[s.a_hi + from]);
-        fa[P ^ 1][f].s = s.sa[sc_a + f * 64];
+        fa[P ^ 1][f].s = s.sa[sc_a + f * 320];
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -412,7 +412,7 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
 }
 
 template <int TA, int TB, int X, int Y, bool DMA>
-__global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product q, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_m, int tiles_n) {
   using S = Slab<X, Y, DMA>;
   __shared__ u32x4 lds[S::CHUNKS];
   const F8Product p = part_of(q, blockIdx.y);
@@ -438,17 +438,12 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   s.put = (8 * wave + r8) * 8 + ((lane & 7) ^ r8);
   s.a_lo = (wi + l16) * 8 + (g ^ (l16 & 7)); s.a_hi = (wi + l16) * 8 + ((g + 4) ^ (l16 & 7));
   s.b_lo = S::B0 + (wj + l16) * 8 + (g ^ (l16 & 7)); s.b_hi = S::B0 + (wj + l16) * 8 + ((g + 4) ^ (l16 & 7));
-  s.sa = (const uint8_t *) (lds + S::S0) + (wi + l16) * 4;
-  s.sb = (const uint8_t *) (lds + S::S0) + (TM + wj + l16) * 4;
-  // scale words: thread t has row t of A (t < TM) and row t of B; with 128 + 128 rows one of them
-  uint32_t *const sw = (uint32_t *) (lds + S::S0) + t;
-  constexpr bool TWO = TM == 256;
-  const uint8_t *const s0_row = t < TM ? p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa : p.sb + (int64_t) ((j0 + t - TM) >> p.b_shift) * p.ldsb;
-  const uint8_t *const s1_row = TWO ? p.sb + (int64_t) ((j0 + min(t, TN - 1)) >> p.b_shift) * p.ldsb : s0_row;
-  auto put_words = [&](int to, uint32_t w0, uint32_t w1, int shift) {
-    sw[to] = w0 >> shift;
-    if (TWO && t < TN) sw[to + TM] = w1 >> shift;
-  };
+  uint8_t *const scales = (uint8_t *) (lds + S::S0);
+  s.sa = scales + (wi + l16) * 20;
+  s.sb = scales + (TM + wj + l16) * 20;
+  // thread t has the scales of row t of A and of row t of B
+  const uint8_t *const sa_row = p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa, *const sb_row = p.sb + (int64_t) ((j0 + t) >> p.b_shift) * p.ldsb;
+  auto half_of = [&](int seg) { return scales + (seg & 1) * (TM + TN) * 20; };
   const uint64_t a_org = reinterpret_cast<uint64_t>(p.a + (int64_t) i0 * p.lda), b_org = reinterpret_cast<uint64_t>(p.b + (int64_t) j0 * p.ldb);
   auto a_at = [&](int kb) { return a_org + (uint64_t) min(kb, full - 1) * 128; };   // (behind the last slab: the last one again)
   auto b_at = [&](int kb) { return b_org + (uint64_t) min(kb, full - 1) * 128; };
@@ -456,7 +451,7 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   {
     const int r = wave * 16 + l16, half = (lane & 32) * 2;
     s.ahead = (lane & 16 ? p.b + (int64_t) (j0 + (tm & 3) * (TN / 4) + r % (TN / 4)) * p.ldb : p.a + (int64_t) (i0 + (tn & 3) * (TM / 4) + r % (TM / 4)) * p.lda) + half;
-    s.junk = lds_address(lds) + (S::S0 + S::WORDS / 2) * 16 + wave * 256;
+    s.junk = lds_address(lds) + S::J0 * 16 + wave * 256;
   }
   f32x4 acc[X][Y];
 #pragma unroll
@@ -488,28 +483,32 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
       lds[s.put + S::B0 + r * 256] = v;
     }
   }
-  // words of the first four blocks (b0 is a multiple of four); of the next four: fetched in front of slab 0 of four, in LDS
-  // before the barrier of slab 2, read from slab 3 on
-  put_words((b0 & 4) ? S::WORDS : 0, scale_word(s0_row, b0, nb), scale_word(s1_row, b0, nb), scale_shift(b0, nb));
+  const int seg = b0 >> 4;
+  {
+    const u32x4 v[4] = {load_chunk(sa_row, seg * 16, nb), load_chunk(sb_row, seg * 16, nb), load_chunk(sa_row, seg * 16 + 16, nb), load_chunk(sb_row, seg * 16 + 16, nb)};
+    put_scales(half_of(seg), t, v[0]);
+    put_scales(half_of(seg), TM + t, v[1]);
+    put_scales(half_of(seg + 1), t, v[2]);
+    put_scales(half_of(seg + 1), TM + t, v[3]);
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  auto byte_of = [](int kb) { return ((kb & 4) ? S::WORDS * 4 : 0) + (kb & 3); };
+  auto byte_of = [](int kb) { return scale_byte(kb, TM + TN); };
 #pragma unroll
   for (int x = 0; x < X; x++) {
     fa[0][x].q = both(lds[s.a_lo + x * 128], lds[s.a_hi + x * 128]);
-    fa[0][x].s = s.sa[byte_of(b0) + x * 64];
+    fa[0][x].s = s.sa[byte_of(b0) + x * 320];
   }
   fb[0].q = both(lds[s.b_lo], lds[s.b_hi]);
   fb[0].s = s.sb[byte_of(b0)];
   __syncthreads();
-  uint32_t w0 = 0, w1 = 0;
-  auto words = [&](int kb) {
-    if ((kb & 3) == 0 && kb + 4 < nb) { w0 = scale_word(s0_row, kb + 4, nb); w1 = scale_word(s1_row, kb + 4, nb); }
-    if ((kb & 3) == 2 && kb + 2 < nb) put_words((~kb & 4) ? S::WORDS : 0, w0, w1, scale_shift(kb + 2, nb));
-  };
   int kb = b0;
   for (; kb + 2 <= full; kb += 2) {
-    words(kb);
+    if ((kb & 15) == 0 && kb > b0) {
+      const u32x4 v[2] = {next_scales(sa_row, kb + 16, nb), next_scales(sb_row, kb + 16, nb)};
+      put_scales(half_of((kb >> 4) + 1), t, v[0]);
+      put_scales(half_of((kb >> 4) + 1), TM + t, v[1]);
+    }
     slab<TA, TB, X, Y, DMA, 0>(s, DMA ? b_at(kb + 1) : b_at(kb + 2), DMA ? a_at(kb + 2) : a_at(kb + 3), ahead_at(kb), byte_of(kb), byte_of(kb + 1), fa, fb, acc);
     slab<TA, TB, X, Y, DMA, 1>(s, DMA ? b_at(kb + 2) : b_at(kb + 3), DMA ? a_at(kb + 3) : a_at(kb + 4), ahead_at(kb + 1), byte_of(kb + 1), byte_of(kb + 2), fa, fb, acc);
   }
@@ -517,31 +516,250 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   if (tail) {   // the short block: through registers, zeros behind k
-#pragma unroll 1
-    for (int u = 0; u < X; u++)
-      lds[s.put + u * 256] = load_chunk(p.a + (int64_t) (i0 + 32 * u + 8 * wave + r8) * p.lda, all * 128 + (lane & 7) * 16, p.k);
-#pragma unroll 1
-    for (int u = 0; u < Y; u++)
-      lds[s.put + S::B0 + u * 256] = load_chunk(p.b + (int64_t) (j0 + 32 * u + 8 * wave + r8) * p.ldb, all * 128 + (lane & 7) * 16, p.k);
-    put_words(0, s0_row[all], s1_row[all], 0);
+    u32x4 v[X + Y];
+#pragma unroll
+    for (int u = 0; u < X + Y; u++)
+      v[u] = load_chunk_of_16(u < X ? p.a + (int64_t) (i0 + 32 * u + 8 * wave + r8) * p.lda : p.b + (int64_t) (j0 + 32 * (u - X) + 8 * wave + r8) * p.ldb,
+                        all * 128 + (lane & 7) * 16, p.k);
+    const uint8_t sa_last = sa_row[all], sb_last = sb_row[all];
+#pragma unroll
+    for (int u = 0; u < X + Y; u++) lds[s.put + (u < X ? u * 256 : S::B0 + (u - X) * 256)] = v[u];
+    scales[t * 20] = sa_last;
+    scales[(TM + t) * 20] = sb_last;
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < X; x++) {
       fa[0][x].q = both(lds[s.a_lo + x * 128], lds[s.a_hi + x * 128]);
-      fa[0][x].s = s.sa[x * 64];
+      fa[0][x].s = s.sa[x * 320];
     }
 #pragma unroll
     for (int y = 0; y < Y; y++) {
       Frag<false> b;
       b.q = both(lds[s.b_lo + y * 128], lds[s.b_hi + y * 128]);
-      b.s = s.sb[y * 64];
+      b.s = s.sb[y * 320];
 #pragma unroll
-      for (int x = 0; x < X; x++) mma_pinned<TA, TB, X * Y == 64>(b, fa[0][x], acc[x][y]);
+      for (int x = 0; x < X; x++) mma_pinned<TA, TB>(b, fa[0][x], acc[x][y]);
     }
     __syncthreads();
   }
   settle();
   store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, max(tm * TM, i0 + wi), max(tn * TN, j0 + wj));
+}
+
+// ---- outputs of few tiles ------------------------------------------------------------
+// Four waves, X x Y tiles of 16 x 16 each: what counts here is not the matrix unit but the way to memory, so LDS is a ring of ST
+// blocks of k.  Step t multiplies block t out of registers, reads the fragments of block t + 1 into the other set of them, and
+// fetches block t + ST into the place that block t has left: a piece has ST - 1 steps to land, a fragment one.  The barrier of a
+// step stands in front of its last MFMAs: by then every wave has read what it wants from LDS, and block t + 2 has landed.  Rows,
+// chunks, scales and the staged form are those of the tiles above (staged: written three blocks ahead, loaded two steps before
+// that); rows behind the last one are read as the last one and not stored.
+//
+// 128 x 128, four blocks, one workgroup a CU: a block takes 0.5 us of it, two thirds of that LDS (64 KB of fragments are read
+// for 32 KB of rows, at 128 bytes a cycle); two images of LDS and two workgroups a CU took 0.8 us on an idle card:
+// 1024 x 4096 x 4096 in 19 us for 28.
+// 128 x 160: the same, for outputs that it covers in fewer rounds of 256 workgroups: 1021 x 5000 x 4100 without padding in 34.6 us for 53
+// (rows of 4100 bytes lie across the L2's lines and cost 5 of them, the short block 4).
+// 64 x 32, six blocks, two workgroups a CU, for few rows and few columns: bound by the bytes of B, 48 x 8192 x 4096 in 8.9 us
+// (3.8 TB/s), 4.8 TB/s at 8 x 8192 x 8192; with eight blocks and one workgroup a CU 128 x 8192 x 4096 took 15.5 us for 12.3.
+template <int X_, int Y_, int WM_, int ST_, bool DMA>
+struct Ring {
+  static constexpr int X = X_, Y = Y_, WM = WM_, WN = 4 / WM, ST = ST_;          // tiles a wave, waves along m and n, blocks in the ring
+  static constexpr int TM = 16 * X * WM, TN = 16 * Y * WN;                       // rows and columns of C
+  static constexpr int B0 = 8 * TM, BLOCK = B0 + 8 * TN, S0 = ST * BLOCK;        // chunks of 16 bytes: B rows, a block, where the scales begin
+  static constexpr int ROWS = TM + TN, CHUNKS = S0 + scale_chunks(ROWS);
+  static constexpr int PA = TM / 32, PIECES = PA + TN / 32;                      // of 32 rows (8 a wave), A's, then B's
+  u32x4 *lds;
+  uint32_t voff[PIECES];         // of this thread's row and chunk
+  uint32_t to;                   // LDS address of this wave's part of a piece in block 0 (DMA)
+  int put;                       // this thread's chunk in a piece (staged)
+  int a_lo, a_hi, b_lo, b_hi;    // this lane's chunks in a block, of tile 0
+  const uint8_t *sa, *sb;        // this lane's scale bytes of tile 0
+  u32x4 staged[2][DMA ? 1 : PIECES];
+};
+
+// Step t, U = its place in the ring; a, b: where the block to fetch begins; sc: the scale byte of block t + 1.
+template <int TA, int TB, bool DMA, int U, class S, int X, int Y>
+__device__ __forceinline__ void ring_step(S &s, uint64_t a, uint64_t b, int sc, Frag<false> (&fa)[2][X], Frag<false> (&fb)[2][Y], f32x4 (&acc)[X][Y]) {
+  constexpr int P = U & 1, N = X * Y, LAST = N - N / 5, WORK = 2 * S::PIECES;   // MFMAs, those in front of the barrier, work beside them
+  static_assert(X + Y == S::PIECES, "a fragment to read for every piece");
+  auto piece = [&](int q) {
+    const uint64_t from = q < S::PA ? a : b;
+    if constexpr (DMA) {
+      dma16(s.voff[q], from, s.to + U * S::BLOCK * 16 + q * 4096);
+    } else {
+      u32x4 &v = s.staged[P][q];
+      s.lds[s.put + (U + 3) % S::ST * S::BLOCK + q * 256] = v;
+      __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(from) + s.voff[q], 16);
+    }
+  };
+  auto read = [&](int f) {   // fragment f of the next block
+    const u32x4 *block = s.lds + (U + 1) % S::ST * S::BLOCK;
+    if (f < Y) {
+      fb[P ^ 1][f].q = both(block[s.b_lo + f * 128], block[s.b_hi + f * 128]);
+      fb[P ^ 1][f].s = s.sb[sc + f * 320];
+    } else {
+      fa[P ^ 1][f - Y].q = both(block[s.a_lo + (f - Y) * 128], block[s.a_hi + (f - Y) * 128]);
+      fa[P ^ 1][f - Y].s = s.sa[sc + (f - Y) * 320];
+    }
+  };
+#pragma unroll
+  for (int at = 0; at <= N; at++) {
+    if (at == LAST) {
+      if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S::ST - 2) * S::PIECES) : "memory");   // block t + 2 has landed
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+    if (at == N) break;
+    mma_pinned<TA, TB>(fb[P][at / X], fa[P][at % X], acc[at % X][at / X]);
+    if (at < LAST) {
+#pragma unroll
+      for (int w = at * WORK / LAST; w < (at + 1) * WORK / LAST; w++) {
+        if (w & 1) read(w >> 1);
+        else piece(w >> 1);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+template <class F, int... U>
+__device__ __forceinline__ void each_place(F &&f, std::integer_sequence<int, U...>) { (f(std::integral_constant<int, U>()), ...); }
+
+template <int TA, int TB, int X, int Y, int WM, int ST, bool DMA>
+__global__ void __launch_bounds__(256, X == 4 ? 1 : 2) f8_ring_kernel(F8Product q, int tiles_m, int tiles_n) {
+  using S = Ring<X, Y, WM, ST, DMA>;
+  __shared__ u32x4 lds[S::CHUNKS];
+  const F8Product p = part_of(q, blockIdx.y);
+  int tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
+  const int i0 = tm * S::TM, j0 = tn * S::TN;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wi = wave / S::WN * 16 * X, wj = wave % S::WN * 16 * Y;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int nb = (p.k + 127) >> 7, all = p.k >> 7;
+  const int b0 = blockIdx.y * p.blocks_per_part, full = min(all, b0 + p.blocks_per_part);   // blocks b0 .. full - 1, one at least
+  const bool tail = nb > all && blockIdx.y == gridDim.y - 1;
+  S s;
+  s.lds = lds;
+  const int r8 = lane >> 3, chunk = (DMA ? (lane & 7) ^ r8 : lane & 7) << 4;
+#pragma unroll
+  for (int r = 0; r < S::PIECES; r++)
+    s.voff[r] = (r < S::PA ? (uint32_t) min(32 * r + 8 * wave + r8, p.m - 1 - i0) * (uint32_t) p.lda
+                           : (uint32_t) min(32 * (r - S::PA) + 8 * wave + r8, p.n - 1 - j0) * (uint32_t) p.ldb) + chunk;
+  s.to = lds_address(lds) + wave * 1024;
+  s.put = (8 * wave + r8) * 8 + ((lane & 7) ^ r8);
+  s.a_lo = (wi + l16) * 8 + (g ^ (l16 & 7)); s.a_hi = (wi + l16) * 8 + ((g + 4) ^ (l16 & 7));
+  s.b_lo = S::B0 + (wj + l16) * 8 + (g ^ (l16 & 7)); s.b_hi = S::B0 + (wj + l16) * 8 + ((g + 4) ^ (l16 & 7));
+  uint8_t *const scales = (uint8_t *) (lds + S::S0);
+  s.sa = scales + (wi + l16) * 20;
+  s.sb = scales + (S::TM + wj + l16) * 20;
+  // thread t has the scales of row t of A and then B, and those of row 256 + t
+  auto scales_of = [&](int row) {
+    return row < S::TM ? p.sa + (int64_t) (min(i0 + row, p.m - 1) >> p.a_shift) * p.ldsa
+                       : p.sb + (int64_t) (min(j0 + min(row - S::TM, S::TN - 1), p.n - 1) >> p.b_shift) * p.ldsb;
+  };
+  const uint8_t *const s_row = scales_of(t), *const s_row2 = S::ROWS > 256 ? scales_of(t + 256) : s_row;
+  auto put_half = [&](int seg, u32x4 v, u32x4 v2) {
+    if (S::ROWS >= 256 || t < S::ROWS) put_scales(scales + (seg & 1) * S::ROWS * 20, t, v);
+    if (S::ROWS > 256 && t < S::ROWS - 256) put_scales(scales + (seg & 1) * S::ROWS * 20, t + 256, v2);
+  };
+  const uint64_t a_org = reinterpret_cast<uint64_t>(p.a + (int64_t) i0 * p.lda), b_org = reinterpret_cast<uint64_t>(p.b + (int64_t) j0 * p.ldb);
+  auto a_at = [&](int kb) { return a_org + (uint64_t) min(kb, full - 1) * 128; };   // (behind the last block: the last one again)
+  auto b_at = [&](int kb) { return b_org + (uint64_t) min(kb, full - 1) * 128; };
+  f32x4 acc[X][Y];
+#pragma unroll
+  for (int x = 0; x < X * Y; x++) acc[x / Y][x % Y] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Frag<false> fa[2][X], fb[2][Y];
+  // the first blocks: as many as fit on their way to LDS; staged: three, and two in registers
+#pragma unroll
+  for (int u = 0; u < (DMA ? S::ST : 3); u++)
+#pragma unroll
+    for (int r = 0; r < S::PIECES; r++) {
+      const uint64_t from = r < S::PA ? a_at(b0 + u) : b_at(b0 + u);
+      if constexpr (DMA) {
+        dma16(s.voff[r], from, s.to + u * S::BLOCK * 16 + r * 4096);
+      } else {
+        u32x4 v;
+        __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(from) + s.voff[r], 16);
+        lds[s.put + u * S::BLOCK + r * 256] = v;
+      }
+    }
+  if constexpr (!DMA) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int r = 0; r < S::PIECES; r++)
+        __builtin_memcpy(&s.staged[u][r], reinterpret_cast<const uint8_t *>(r < S::PA ? a_at(b0 + 3 + u) : b_at(b0 + 3 + u)) + s.voff[r], 16);
+  }
+  int seg = b0 >> 4;   // LDS has the scales of blocks 16 seg .. 16 seg + 31
+  {
+    const u32x4 v0 = load_chunk(s_row, seg * 16, nb), v1 = load_chunk(s_row, seg * 16 + 16, nb);
+    u32x4 w0 = v0, w1 = v1;
+    if constexpr (S::ROWS > 256) { w0 = load_chunk(s_row2, seg * 16, nb); w1 = load_chunk(s_row2, seg * 16 + 16, nb); }
+    put_half(seg, v0, w0);
+    put_half(seg + 1, v1, w1);
+  }
+  if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S::ST - 2) * S::PIECES) : "memory");   // the first two blocks (and the scales)
+  __syncthreads();
+  auto byte_of = [](int kb) { return scale_byte(kb, S::ROWS); };
+  auto fragments = [&](int sc) {
+#pragma unroll
+    for (int x = 0; x < X; x++) {
+      fa[0][x].q = both(lds[s.a_lo + x * 128], lds[s.a_hi + x * 128]);
+      fa[0][x].s = s.sa[sc + x * 320];
+    }
+#pragma unroll
+    for (int y = 0; y < Y; y++) {
+      fb[0][y].q = both(lds[s.b_lo + y * 128], lds[s.b_hi + y * 128]);
+      fb[0][y].s = s.sb[sc + y * 320];
+    }
+  };
+  fragments(byte_of(b0));
+  __syncthreads();
+  int kb = b0;
+  auto next = [&](auto place) {   // one step, at its place in the ring
+    constexpr int U = decltype(place)::value, AHEAD = DMA ? ST : 5;
+    ring_step<TA, TB, DMA, U>(s, a_at(kb + AHEAD), b_at(kb + AHEAD), byte_of(kb + 1), fa, fb, acc);
+    kb++;
+  };
+  auto more_scales = [&] {        // the half that is read for the first time ten steps later at the earliest
+    if (kb >> 4 == seg) return;
+    seg++;
+    const u32x4 v = next_scales(s_row, seg * 16 + 16, nb);
+    u32x4 w = v;
+    if constexpr (S::ROWS > 256) w = next_scales(s_row2, seg * 16 + 16, nb);
+    put_half(seg + 1, v, w);
+  };
+  while (kb + ST <= full) {
+    more_scales();
+    each_place(next, std::make_integer_sequence<int, ST>());
+  }
+  more_scales();
+  each_place([&](auto place) { if (kb < full) next(place); }, std::make_integer_sequence<int, ST - 1>());
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tail) {   // the short block: through registers, zeros behind k
+    u32x4 v[S::PIECES];
+#pragma unroll
+    for (int r = 0; r < S::PIECES; r++) {
+      const int row = (r < S::PA ? r : r - S::PA) * 32 + 8 * wave + r8;
+      v[r] = load_chunk_of_16(r < S::PA ? p.a + (int64_t) min(i0 + row, p.m - 1) * p.lda : p.b + (int64_t) min(j0 + row, p.n - 1) * p.ldb,
+                              all * 128 + (lane & 7) * 16, p.k);
+    }
+    const uint8_t s_last = s_row[all], s_last2 = s_row2[all];
+#pragma unroll
+    for (int r = 0; r < S::PIECES; r++) lds[s.put + r * 256] = v[r];
+    if (t < S::ROWS) scales[t * 20] = s_last;
+    if (S::ROWS > 256 && t < S::ROWS - 256) scales[(t + 256) * 20] = s_last2;
+    __syncthreads();
+    fragments(0);
+#pragma unroll
+    for (int at = 0; at < X * Y; at++) mma_pinned<TA, TB>(fb[0][at / X], fa[0][at % X], acc[at % X][at / X]);
+    __syncthreads();
+  }
+  settle();
+  store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, 0, 0);
 }
 
 // ---- tiles, wide ---------------------------------------------------------------------
@@ -550,13 +768,16 @@ __global__ void __launch_bounds__(256, X == 8 ? 1 : 2) f8_tile_kernel(F8Product 
 // owns 32 X rows and 128 columns of C, waves 0-3 work on the first half of every block of k, waves 4-7 on the second, each
 // with sums of its own that are added in the end.
 //
-// LDS: three slots of one block (A and B rows of 128 bytes, swizzled as above) and the scale words.  Step t multiplies block t
+// LDS: three slots of one block (A and B rows of 128 bytes, swizzled as above) and the scales.  Step t multiplies block t
 // out of registers, reads block t + 1 into them -- every fragment as soon as its predecessor is widened -- and fetches block
 // t + 3 into the slot that block t has left: a piece has two steps to land, a fragment one.  A barrier ends each step.
+//
+// 256 x 128, X = 8: 4096 x 2048 x 16384 in 224 us (1.23 PFLOP/s): the matrix unit, at the clock that the card's power leaves it, and
+// the conversions that do not fit beside it.  128 x 128, X = 4, for outputs of few tiles: 128 x 4096 x 4096 in 19.6 us.
 template <int X>
 struct WideSlab {
   static constexpr int A_IMAGE = 256 * X, SLOT = A_IMAGE + 1024;   // chunks of 16 bytes
-  static constexpr int S0 = 3 * SLOT, WORDS = 32 * X + 128, CHUNKS = S0 + WORDS / 2;
+  static constexpr int S0 = 3 * SLOT, ROWS = 32 * X + 128, CHUNKS = S0 + scale_chunks(ROWS);
   static constexpr int PIECES = (X + 4) / 2;                       // of 64 rows (8 a wave)
 };
 
@@ -568,7 +789,9 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   constexpr int TM = 32 * X, TN = 128, Y = 4;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
-  const int i0 = min(tm * TM, p.m - TM), j0 = min(tn * TN, p.n - TN);
+  // (X = 8 has a whole tile at least; with X = 4 rows behind the last one are read as the last one and not stored)
+  constexpr bool CLAMP = X == 4;
+  const int i0 = CLAMP ? tm * TM : min(tm * TM, p.m - TM), j0 = CLAMP ? tn * TN : min(tn * TN, p.n - TN);
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), group = wave >> 2;
   const int wi = ((wave >> 1) & 1) * 16 * X, wj = (wave & 1) * 64;
   const int l16 = lane & 15, g = lane >> 4;
@@ -578,7 +801,12 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   // piece r: rows 64 r + 8 wave + lane / 8 of A and then B
   const int r8 = lane >> 3, chunk = (DMA ? (lane & 7) ^ r8 : lane & 7) << 4;
   const uint32_t a_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.lda + chunk, b_voff = (uint32_t) (8 * wave + r8) * (uint32_t) p.ldb + chunk;
-  const uint64_t a_step = (uint64_t) p.lda * 64, b_step = (uint64_t) p.ldb * 64;
+  uint32_t voff[CLAMP ? S::PIECES : 1];
+#pragma unroll
+  for (int r = 0; CLAMP && r < S::PIECES; r++)
+    voff[r] = (r < X / 2 ? (uint32_t) min(64 * r + 8 * wave + r8, p.m - 1 - i0) * (uint32_t) p.lda
+                         : (uint32_t) min(64 * (r - X / 2) + 8 * wave + r8, p.n - 1 - j0) * (uint32_t) p.ldb) + chunk;
+  const uint64_t a_step = CLAMP ? 0 : (uint64_t) p.lda * 64, b_step = CLAMP ? 0 : (uint64_t) p.ldb * 64;
   const uint64_t a_org = reinterpret_cast<uint64_t>(p.a + (int64_t) i0 * p.lda), b_org = reinterpret_cast<uint64_t>(p.b + (int64_t) j0 * p.ldb);
   const uint32_t to = lds_address(lds) + wave * 1024;
   const int put = (8 * wave + r8) * 8 + ((lane & 7) ^ r8);
@@ -588,8 +816,9 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
     for (int r = 0; r < S::PIECES; r++) {
       const bool a = r < X / 2;
       const uint64_t from = (a ? a_org + r * a_step : b_org + (r - X / 2) * b_step) + (uint64_t) min(blk, full - 1) * 128;
-      if constexpr (DMA) dma16(a ? a_voff : b_voff, from, to + slot * S::SLOT * 16 + r * 8192);
-      else __builtin_memcpy(&staged[r], reinterpret_cast<const uint8_t *>(from) + (a ? a_voff : b_voff), 16);
+      const uint32_t off = CLAMP ? voff[CLAMP ? r : 0] : a ? a_voff : b_voff;
+      if constexpr (DMA) dma16(off, from, to + slot * S::SLOT * 16 + r * 8192);
+      else __builtin_memcpy(&staged[r], reinterpret_cast<const uint8_t *>(from) + off, 16);
     }
   };
   auto land = [&](int slot) {             // ... and there (staged)
@@ -598,14 +827,15 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
       for (int r = 0; r < S::PIECES; r++) lds[slot * S::SLOT + put + r * 512] = staged[r];
     }
   };
-  // scale words: thread t has row t of A and then B
-  uint32_t *const sw = (uint32_t *) (lds + S::S0) + t;
-  const uint8_t *const s_row = t < TM ? p.sa + (int64_t) ((i0 + t) >> p.a_shift) * p.ldsa : p.sb + (int64_t) ((j0 + min(t - TM, TN - 1)) >> p.b_shift) * p.ldsb;
-  auto put_word = [&](int at, uint32_t w) { if (t < S::WORDS) sw[at] = w; };
+  // thread t has the scales of row t of A and then B
+  uint8_t *const scales = (uint8_t *) (lds + S::S0);
+  const uint8_t *const s_row = t < TM ? p.sa + (int64_t) (min(i0 + t, p.m - 1) >> p.a_shift) * p.ldsa
+                                      : p.sb + (int64_t) (min(j0 + min(t - TM, TN - 1), p.n - 1) >> p.b_shift) * p.ldsb;
+  auto put_half = [&](int seg, u32x4 v) { if (t < S::ROWS) put_scales(scales + (seg & 1) * S::ROWS * 20, t, v); };
   // this lane's chunk in an image, of tile 0: its half of the block
   const int a_at = (wi + l16) * 8 + ((4 * group + g) ^ (l16 & 7)), b_at = S::A_IMAGE + (wj + l16) * 8 + ((4 * group + g) ^ (l16 & 7));
-  const uint8_t *const sa = (const uint8_t *) (lds + S::S0) + (wi + l16) * 4, *const sb = (const uint8_t *) (lds + S::S0) + (TM + wj + l16) * 4;
-  auto byte_of = [](int kb) { return ((kb & 4) ? S::WORDS * 4 : 0) + (kb & 3); };
+  const uint8_t *const sa = scales + (wi + l16) * 20, *const sb = scales + (TM + wj + l16) * 20;
+  auto byte_of = [](int kb) { return scale_byte(kb, S::ROWS); };
   f32x4 acc[X][Y];
 #pragma unroll
   for (int x = 0; x < X * Y; x++) acc[x / Y][x % Y] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -616,14 +846,14 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
     const u32x4 *const img = lds + next * S::SLOT;
 #pragma unroll
     for (int y = 0; y < Y; y++) {
-      const float sc = scale_value(sb[byte + y * 64]);
+      const float sc = scale_value(sb[byte + y * 320]);
       b[y][0] = widen8<TB>((int) rb[y][0], (int) rb[y][1], sc);
       b[y][1] = widen8<TB>((int) rb[y][2], (int) rb[y][3], sc);
       rb[y] = img[b_at + y * 128];
     }
 #pragma unroll
     for (int x = 0; x < X; x++) {
-      const float sc = scale_value(sa[byte + x * 64]);
+      const float sc = scale_value(sa[byte + x * 320]);
       const bf16x8 a0 = widen8<TA>((int) ra[x][0], (int) ra[x][1], sc), a1 = widen8<TA>((int) ra[x][2], (int) ra[x][3], sc);
       ra[x] = img[a_at + x * 128];
 #pragma unroll
@@ -642,20 +872,22 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   fetch(b0, 0); land(0);
   fetch(b0 + 1, 1); land(1);
   fetch(b0 + 2, 2);
-  put_word((b0 & 4) ? S::WORDS : 0, scale_word(s_row, b0, nb) >> scale_shift(b0, nb));
+  {
+    const int seg = b0 >> 4;
+    const u32x4 v0 = load_chunk(s_row, seg * 16, nb), v1 = load_chunk(s_row, seg * 16 + 16, nb);
+    put_half(seg, v0);
+    put_half(seg + 1, v1);
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   read_first(0);
-  uint32_t word = 0;
   int slot = 0;   // of block kb
   for (int kb = b0; kb < full; kb++) {
-    // the scales of the next four blocks (b0 is a multiple of four): fetched in step 0 of four, in LDS by the end of step 2
-    if ((kb & 3) == 0 && kb + 4 < nb) word = scale_word(s_row, kb + 4, nb);
+    if ((kb & 15) == 0 && kb > b0) put_half((kb >> 4) + 1, next_scales(s_row, kb + 16, nb));
     const int next = slot == 2 ? 0 : slot + 1;
     if constexpr (!DMA) land(next == 2 ? 0 : next + 1);   // (block kb + 2, fetched in the step before)
     fetch(kb + 3, slot);
     multiply(next, byte_of(kb));
-    if ((kb & 3) == 2 && kb + 2 < nb) put_word((~kb & 4) ? S::WORDS : 0, word >> scale_shift(kb + 2, nb));
     if constexpr (DMA) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(S::PIECES) : "memory");   // block kb + 2 has landed
     __syncthreads();
     slot = next;
@@ -663,13 +895,17 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tail) {   // the short block: through registers, zeros behind k
-#pragma unroll 1
+    u32x4 v[S::PIECES];
+#pragma unroll
     for (int u = 0; u < S::PIECES; u++) {
       const int r = 64 * u + 8 * wave + r8;
-      const uint8_t *row = u < X / 2 ? p.a + (int64_t) (i0 + r) * p.lda : p.b + (int64_t) (j0 + r - TM) * p.ldb;
-      lds[put + u * 512] = load_chunk(row, all * 128 + (lane & 7) * 16, p.k);
+      v[u] = load_chunk_of_16(u < X / 2 ? p.a + (int64_t) min(i0 + r, p.m - 1) * p.lda : p.b + (int64_t) min(j0 + r - TM, p.n - 1) * p.ldb,
+                              all * 128 + (lane & 7) * 16, p.k);
     }
-    put_word(0, s_row[all]);
+    const uint8_t s_last = s_row[all];
+#pragma unroll
+    for (int u = 0; u < S::PIECES; u++) lds[put + u * 512] = v[u];
+    if (t < S::ROWS) scales[t * 20] = s_last;
     __syncthreads();
     read_first(0);
     multiply(0, 0);
@@ -696,90 +932,96 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
 }
 
 // ---- few rows of A -------------------------------------------------------------------
-// Up to 64 rows of A: the bytes of B bound the product.  A workgroup owns 16 NT columns of C and all of k; its waves take the
-// blocks of k in turn, so that every wave streams B (and A, from the caches) straight into registers, UNROLL blocks in
-// flight, and nobody waits for anybody until the waves' sums are added, in their order, through LDS.
+// Up to 16 rows of A, 32 of a wide product: the bytes of B bound it.  A workgroup owns 16 NT columns of C and all of k; its waves
+// take the blocks of k in turn, so that every wave streams B straight into registers, four blocks in flight (and A, from the
+// caches, two), and nobody waits for anybody until the waves' sums are added, in their order, through LDS.  1 x 4096 x 4096 in
+// 5.9 us (2.8 TB/s, 2.5 us of it the launch), wide 32 x 4096 x 4096 in 12.0.
 template <int TA, int TB, bool WIDE, int MT, int NT>
 __global__ void __launch_bounds__(512) f8_rows_kernel(F8Product p) {
   extern __shared__ f32x4 sums[];   // [wave][tile][lane]
-  constexpr int UNROLL = MT == 4 ? 1 : 2;
+  constexpr int DEEP = 4;           // blocks of B in flight a wave
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6;
   const int l16 = lane & 15, g = lane >> 4, j0 = blockIdx.x * 16 * NT;
   const int full = p.k >> 7;
-  const uint8_t *a_row[MT], *b_row[NT], *sa_row[MT], *sb_row[NT];
+  // (offsets of 32 bits from where the workgroup's rows begin: half the registers that pointers would take)
+  const uint8_t *const b0 = p.b + (int64_t) j0 * p.ldb, *const sb0 = p.sb + (int64_t) (j0 >> p.b_shift) * p.ldsb;
+  uint32_t a_off[MT], b_off[NT], sa_off[MT], sb_off[NT];
 #pragma unroll
   for (int x = 0; x < MT; x++) {
     const int i = min(x * 16 + l16, p.m - 1);
-    a_row[x] = p.a + i * p.lda + g * 16;
-    sa_row[x] = p.sa + (i >> p.a_shift) * p.ldsa;
+    a_off[x] = (uint32_t) i * (uint32_t) p.lda + g * 16;
+    sa_off[x] = (uint32_t) (i >> p.a_shift) * (uint32_t) p.ldsa;
   }
 #pragma unroll
   for (int y = 0; y < NT; y++) {
     const int j = min(j0 + y * 16 + l16, p.n - 1);
-    b_row[y] = p.b + j * p.ldb + g * 16;
-    sb_row[y] = p.sb + (j >> p.b_shift) * p.ldsb;
+    b_off[y] = (uint32_t) (j - j0) * (uint32_t) p.ldb + g * 16;
+    sb_off[y] = (uint32_t) ((j >> p.b_shift) - (j0 >> p.b_shift)) * (uint32_t) p.ldsb;
   }
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int x = 0; x < MT * NT; x++) acc[x / NT][x % NT] = f32x4{0.f, 0.f, 0.f, 0.f};
-  struct Block {
-    u32x4 a[MT][2], b[NT][2];
-    uint8_t sa[MT], sb[NT];
-  };
-  auto fetch = [&](Block &v, int blk) {
-    const int64_t at = (int64_t) blk * 128;
-#pragma unroll
-    for (int y = 0; y < NT; y++) {
-      __builtin_memcpy(&v.b[y][0], b_row[y] + at, 16);
-      __builtin_memcpy(&v.b[y][1], b_row[y] + at + 64, 16);
-      v.sb[y] = sb_row[y][blk];
-    }
+  struct BlockA { u32x4 q[MT][2]; uint8_t s[MT]; };
+  struct BlockB { u32x4 q[NT][2]; uint8_t s[NT]; };
+  auto fetch_a = [&](BlockA &v, int blk) {
 #pragma unroll
     for (int x = 0; x < MT; x++) {
-      __builtin_memcpy(&v.a[x][0], a_row[x] + at, 16);
-      __builtin_memcpy(&v.a[x][1], a_row[x] + at + 64, 16);
-      v.sa[x] = sa_row[x][blk];
+      const uint8_t *from = p.a + (int64_t) blk * 128 + a_off[x];
+      __builtin_memcpy(&v.q[x][0], from, 16);
+      __builtin_memcpy(&v.q[x][1], from + 64, 16);
+      v.s[x] = (p.sa + blk)[sa_off[x]];
     }
   };
-  auto multiply = [&](const Block &v) {
-    Frag<WIDE> fa[MT];
-#pragma unroll
-    for (int x = 0; x < MT; x++) fa[x] = make_frag<TA, WIDE>(v.a[x][0], v.a[x][1], v.sa[x]);
+  auto fetch_b = [&](BlockB &v, int blk) {
 #pragma unroll
     for (int y = 0; y < NT; y++) {
-      const Frag<WIDE> fb = make_frag<TB, WIDE>(v.b[y][0], v.b[y][1], v.sb[y]);
+      const uint8_t *from = b0 + (int64_t) blk * 128 + b_off[y];
+      __builtin_memcpy(&v.q[y][0], from, 16);
+      __builtin_memcpy(&v.q[y][1], from + 64, 16);
+      v.s[y] = (sb0 + blk)[sb_off[y]];
+    }
+  };
+  auto multiply = [&](const BlockA &a, const BlockB &b) {
+    Frag<WIDE> fa[MT];
+#pragma unroll
+    for (int x = 0; x < MT; x++) fa[x] = make_frag<TA, WIDE>(a.q[x][0], a.q[x][1], a.s[x]);
+#pragma unroll
+    for (int y = 0; y < NT; y++) {
+      const Frag<WIDE> fb = make_frag<TB, WIDE>(b.q[y][0], b.q[y][1], b.s[y]);
 #pragma unroll
       for (int x = 0; x < MT; x++) acc[x][y] = mma<TA, TB, WIDE>(fb, fa[x], acc[x][y]);
     }
   };
-  int blk = wave;
-  for (; blk + (UNROLL - 1) * waves < full; blk += UNROLL * waves) {
-    Block v[UNROLL];
+  // (blocks behind the last one: the last one again, not multiplied)
+  for (int blk = wave; blk < full; blk += DEEP * waves) {
+    BlockB b[DEEP];
+    BlockA a[2];
 #pragma unroll
-    for (int u = 0; u < UNROLL; u++) fetch(v[u], blk + u * waves);
+    for (int u = 0; u < DEEP; u++) fetch_b(b[u], min(blk + u * waves, full - 1));
+    fetch_a(a[0], blk);
 #pragma unroll
-    for (int u = 0; u < UNROLL; u++) multiply(v[u]);
-  }
-  for (; blk < full; blk += waves) {
-    Block v;
-    fetch(v, blk);
-    multiply(v);
+    for (int u = 0; u < DEEP; u++) {
+      if (u + 1 < DEEP) fetch_a(a[(u + 1) & 1], min(blk + (u + 1) * waves, full - 1));
+      __builtin_amdgcn_sched_barrier(0);
+      if (blk + u * waves < full) multiply(a[u & 1], b[u]);
+    }
   }
   if ((p.k & 127) && wave == full % waves) {   // the short block
-    Block v;
-#pragma unroll
-    for (int y = 0; y < NT; y++) {
-      v.b[y][0] = load_chunk(b_row[y] - g * 16, full * 128 + g * 16, p.k);
-      v.b[y][1] = load_chunk(b_row[y] - g * 16, full * 128 + g * 16 + 64, p.k);
-      v.sb[y] = sb_row[y][full];
-    }
+    BlockA a;
+    BlockB b;
 #pragma unroll
     for (int x = 0; x < MT; x++) {
-      v.a[x][0] = load_chunk(a_row[x] - g * 16, full * 128 + g * 16, p.k);
-      v.a[x][1] = load_chunk(a_row[x] - g * 16, full * 128 + g * 16 + 64, p.k);
-      v.sa[x] = sa_row[x][full];
+      a.q[x][0] = load_chunk(p.a + a_off[x] - g * 16, full * 128 + g * 16, p.k);
+      a.q[x][1] = load_chunk(p.a + a_off[x] - g * 16, full * 128 + g * 16 + 64, p.k);
+      a.s[x] = (p.sa + full)[sa_off[x]];
     }
-    multiply(v);
+#pragma unroll
+    for (int y = 0; y < NT; y++) {
+      b.q[y][0] = load_chunk(b0 + b_off[y] - g * 16, full * 128 + g * 16, p.k);
+      b.q[y][1] = load_chunk(b0 + b_off[y] - g * 16, full * 128 + g * 16 + 64, p.k);
+      b.s[y] = (sb0 + full)[sb_off[y]];
+    }
+    multiply(a, b);
   }
 #pragma unroll
   for (int x = 0; x < MT * NT; x++) sums[(wave * MT * NT + x) * 64 + lane] = acc[x / NT][x % NT];
@@ -797,7 +1039,7 @@ __global__ void __launch_bounds__(512) f8_rows_kernel(F8Product p) {
   }
 }
 
-// C from the parts of the sums, added in their order (no parts: C = beta * C)
+// C from the parts of the sums, added in their order (no parts: C = beta * C).  Bound by its launch, 4 us, and the parts' bytes.
 __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
   const int64_t mn = (int64_t) p.m * p.n;
   if (p.n % 8 == 0) {   // eight neighbours a thread
@@ -823,27 +1065,70 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
 }
 
 // ---- which kernel --------------------------------------------------------------------
+enum Kind { kAny, kRows, kRing64, kRing128, kRing160, kTile256, kWide128, kWide256 };
+struct Plan {
+  Kind kind;
+  int parts;   // along k
+};
 constexpr int kMaxParts = 32;
 
-// Parts along k: workgroups of 128 x 128 to give every one of the 256 compute units two, each with eight blocks of k at least
-// (the join reads and writes every part again: it pays for itself from about 24 blocks on).
-int wanted_parts(int64_t m, int64_t n, int64_t k) {
-  const int64_t tiles = ((m + 127) / 128) * ((n + 127) / 128), nb = (k + 127) / 128;
-  if (m <= 64 || nb < 24) return 1;
-  const int64_t parts = 512 / tiles < nb / 8 ? 512 / tiles : nb / 8;
-  return (int) (parts < 1 ? 1 : parts > kMaxParts ? kMaxParts : parts);
+// The kernel, and the parts along k, of least time by this estimate: us that a block of k takes a CU that holds one workgroup, the
+// same for two of them (0: it holds one), and 3 us; for parts a join of 4 us and 4 TB/s for what they write and it reads.
+//   64 x 32      one workgroup a CU 0.16, two 0.30     48 x 8192 x 4096 9 us, 128 x 8192 x 4096 12 (128 x 128: 14 and 17)
+//   128 x 128    0.50                                  1024 x 4096 x 4096 20 us (64 x 32: 40, 256 x 256: 45)
+//   128 x 160    0.64                                  1024 x 5120 x 4096 24 us (128 x 128: 34, 256 x 256: 46)
+//   256 x 256    1.35                                  4096 x 4096 x 4096 56 us (128 x 128: 76)
+//   wide         0.9 (128 x 128), 1.7 (256 x 128)
+// One to sixteen rows of A and a workgroup a CU at most go to the kernel for few rows: 1 x 4096 x 4096 in 5.9 us, in 7.5 by tiles
+// of 64 x 32; 8 x 4096 x 8192 in 10.8 and 11.1; 1 x 8192 x 4096 in 8.8 and 8.4, 1 x 512 x 16384 in 11.9 and 9.0.  Wide: all up to
+// 32 rows, 32 x 4096 x 4096 in 12.0 us (33 rows by tiles: 15.6).
+Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, int max_parts) {
+  if (m <= 16 && n <= 4096 && k <= 8192 && near) return {kRows, 1};
+  if (wide && m <= 32 && n <= (1 << 26) && near) return {kRows, 1};
+  if (k < 128 || !near) return {kAny, 1};
+  const int64_t nb = k / 128;
+  Plan best{kAny, 1};
+  double least = 1e30;
+  auto consider = [&](Kind kind, int tm, int tn, double one, double two) {
+    const int64_t tiles = ((m + tm - 1) / tm) * ((n + tn - 1) / tn);
+    for (int64_t parts = 1; parts <= max_parts && (parts == 1 || (parts * tiles <= (two > 0 ? 512 : 256) && parts * 8 <= nb + 7)); parts++) {
+      const int64_t all = tiles * parts, rest = all % 512;
+      const double rounds = two > 0 ? (double) (all / 512) * two + (rest == 0 ? 0 : rest <= 256 ? one : two) : (double) ((all + 255) / 256) * one;
+      const double us = (double) ((nb + parts - 1) / parts) * rounds + 3 + (parts > 1 ? 4 + (double) parts * (double) m * (double) n * 8 / 4e6 : 0);
+      if (us < least) { least = us; best = {kind, (int) parts}; }
+    }
+  };
+  if (wide) {
+    consider(kWide128, 128, 128, 0.9, 0);
+    if (m >= 256 && n >= 128) consider(kWide256, 256, 128, 1.7, 0);
+  } else {
+    consider(kRing64, 64, 32, 0.16, 0.30);
+    consider(kRing128, 128, 128, 0.50, 0);
+    consider(kRing160, 128, 160, 0.64, 0);
+    if (m >= 256 && n >= 256) max_parts = 1, consider(kTile256, 256, 256, 1.35, 0);
+  }
+  return best;
 }
 
+// what the DMA to LDS needs of a row: 16-byte chunks at multiples of four bytes (at no loss: reads from the L2 run at 20 TB/s at any
+// such address, at 10 at odd ones)
 bool rows_aligned(const F8Product &p) {
-  return p.lda % 16 == 0 && p.ldb % 16 == 0 && reinterpret_cast<uintptr_t>(p.a) % 16 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0;
+  return p.lda % 4 == 0 && p.ldb % 4 == 0 && reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % 4 == 0;
 }
 
-template <int TA, int TB, int X, int Y>
-void start_tiles(const F8Product &p, int parts, hipStream_t st) {
-  const int tiles_m = (p.m + 32 * X - 1) / (32 * X), tiles_n = (p.n + 32 * Y - 1) / (32 * Y);
+template <int TA, int TB>
+void start_tiles(const F8Product &p, hipStream_t st) {
+  const int tiles_m = (p.m + 255) / 256, tiles_n = (p.n + 255) / 256;
+  if (rows_aligned(p)) f8_tile_kernel<TA, TB, 8, 8, true><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
+  else f8_tile_kernel<TA, TB, 8, 8, false><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
+}
+template <int TA, int TB, int X, int Y, int WM, int ST>
+void start_ring(const F8Product &p, int parts, hipStream_t st) {
+  using S = Ring<X, Y, WM, ST, true>;
+  const int tiles_m = (p.m + S::TM - 1) / S::TM, tiles_n = (p.n + S::TN - 1) / S::TN;
   const dim3 grid((unsigned) (tiles_m * tiles_n), (unsigned) parts);
-  if (rows_aligned(p)) f8_tile_kernel<TA, TB, X, Y, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
-  else f8_tile_kernel<TA, TB, X, Y, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
+  if (rows_aligned(p)) f8_ring_kernel<TA, TB, X, Y, WM, ST, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
+  else f8_ring_kernel<TA, TB, X, Y, WM, ST, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 
 template <int TA, int TB, int X>
@@ -854,41 +1139,39 @@ void start_wide(const F8Product &p, int parts, hipStream_t st) {
   else f8_wide_kernel<TA, TB, X, false><<<grid, 512, 0, st>>>(p, tiles_m, tiles_n);
 }
 
-template <int TA, int TB, int MT, int NT>
+template <int TA, int TB, bool WIDE, int MT, int NT>
 void start_rows(const F8Product &p, hipStream_t st) {
   const int waves = 8;
   const unsigned wg = (unsigned) ((p.n + 16 * NT - 1) / (16 * NT)), bytes = waves * MT * NT * 1024;
-  if (p.c_type == BOF_F32) f8_rows_kernel<TA, TB, true, MT, NT><<<wg, 64 * waves, bytes, st>>>(p);
-  else f8_rows_kernel<TA, TB, false, MT, NT><<<wg, 64 * waves, bytes, st>>>(p);
+  f8_rows_kernel<TA, TB, WIDE, MT, NT><<<wg, 64 * waves, bytes, st>>>(p);
 }
 
 template <int TA, int TB>
-hipError_t launch_product(F8Product p, int parts, hipStream_t st) {
-  // parts begin at multiples of four blocks; the short block is the last part's
-  const int all = p.k < 128 ? 1 : p.k / 128;
-  p.blocks_per_part = ((all + parts - 1) / parts + 3) & ~3;
-  parts = (all + p.blocks_per_part - 1) / p.blocks_per_part;
+hipError_t launch_product(F8Product p, Plan plan, hipStream_t st) {
+  // the short block is the last part's
+  const int all = p.k / 128 ? p.k / 128 : 1;
+  p.blocks_per_part = (all + plan.parts - 1) / plan.parts;
+  const int parts = (all + p.blocks_per_part - 1) / p.blocks_per_part;
   if (parts == 1) p.part = nullptr;
-  const auto tiles = [&](int e) { return ((p.m + e - 1) / e) * (int64_t) ((p.n + e - 1) / e); };
   drop_stale_error();
-  if (p.m <= 64 && p.n <= (1 << 26)) {   // (more columns: more threads than a launch holds)
-    if (p.m <= 16) start_rows<TA, TB, 1, 1>(p, st);
-    else if (p.m <= 32) start_rows<TA, TB, 2, 2>(p, st);
-    else start_rows<TA, TB, 4, 2>(p, st);
-    return hipGetLastError();
-  }
-  if (p.c_type != BOF_F32 && p.m >= 128 && p.n >= 128 && p.k >= 128 && p.lda <= (1 << 26) && p.ldb <= (1 << 26)) {
-    // a slab of 256 x 256 takes a CU about 2200 cycles, one of 128 x 128 about 770
-    const int64_t t256 = (tiles(256) + 255) / 256 * 2200, t128 = (tiles(128) + 255) / 256 * 770;
-    if (parts == 1 && p.m >= 256 && p.n >= 256 && t256 <= t128) start_tiles<TA, TB, 8, 8>(p, 1, st);
-    else start_tiles<TA, TB, 4, 4>(p, parts, st);
-  } else if (p.c_type == BOF_F32 && p.m >= 128 && p.n >= 128 && p.k >= 128 && p.lda <= (1 << 25) && p.ldb <= (1 << 25)) {
-    if (p.m >= 256) start_wide<TA, TB, 8>(p, parts, st);
-    else start_wide<TA, TB, 4>(p, parts, st);
-  } else {
-    const dim3 grid((unsigned) tiles(128), (unsigned) parts);
-    if (p.c_type == BOF_F32) f8_tile_any_kernel<TA, TB, true><<<grid, 256, 0, st>>>(p);
-    else f8_tile_any_kernel<TA, TB, false><<<grid, 256, 0, st>>>(p);
+  switch (plan.kind) {
+    case kAny: {
+      const unsigned tiles = (unsigned) (((p.m + 127) / 128) * (int64_t) ((p.n + 127) / 128));
+      if (p.c_type == BOF_F32) f8_tile_any_kernel<TA, TB, true><<<tiles, 256, 0, st>>>(p);
+      else f8_tile_any_kernel<TA, TB, false><<<tiles, 256, 0, st>>>(p);
+      break;
+    }
+    case kRows:
+      if (p.c_type != BOF_F32) start_rows<TA, TB, false, 1, 1>(p, st);
+      else if (p.m <= 16) start_rows<TA, TB, true, 1, 1>(p, st);
+      else start_rows<TA, TB, true, 2, 2>(p, st);
+      break;
+    case kRing64: start_ring<TA, TB, 2, 1, 2, 6>(p, parts, st); break;
+    case kRing128: start_ring<TA, TB, 4, 4, 2, 4>(p, parts, st); break;
+    case kRing160: start_ring<TA, TB, 4, 5, 2, 4>(p, parts, st); break;
+    case kTile256: start_tiles<TA, TB>(p, st); break;
+    case kWide128: start_wide<TA, TB, 4>(p, parts, st); break;
+    case kWide256: start_wide<TA, TB, 8>(p, parts, st); break;
   }
   if (parts > 1) {
     const int64_t wg = ((int64_t) p.m * p.n + 255) / 256;
@@ -907,7 +1190,8 @@ extern "C" {
 
 uint64_t bof_f8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0 || m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return 0;
-  const int parts = wanted_parts(m, n, k);
+  const int narrow = plan_product(m, n, k, false, true, kMaxParts).parts, wide = plan_product(m, n, k, true, true, kMaxParts).parts;
+  const int parts = narrow > wide ? narrow : wide;
   return parts > 1 ? (uint64_t) parts * (uint64_t) m * (uint64_t) n * 4u : 0;
 }
 
@@ -943,18 +1227,18 @@ int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int
   }
   for (auto [q, name] : {std::pair<const void *, const char *>{a, "A"}, {b, "B"}, {sa, "sa"}, {sb, "sb"}})
     if (int rc = dev.reaches(q, kCall, name)) return rc;
-  int parts = wanted_parts(m, n, k);
-  const uint64_t one = (uint64_t) m * (uint64_t) n * 4u;
-  if (!work || work_bytes / one < (uint64_t) parts) parts = work ? (int) (work_bytes / one) : 1;
-  if (parts < 2) parts = 1;
-  else if (int rc = dev.reaches(work, kCall, "work")) return rc;
+  const uint64_t room = work ? work_bytes / ((uint64_t) m * (uint64_t) n * 4u) : 0;
+  const bool near = lda <= (1 << 24) && ldb <= (1 << 24) && ldsa <= (1 << 24) && ldsb <= (1 << 24);   // a tile of 256 rows: offsets of 32 bits
+  const Plan plan = plan_product(m, n, k, c_type == BOF_F32, near, room < 2 ? 1 : room < kMaxParts ? (int) room : kMaxParts);
+  if (plan.parts > 1)
+    if (int rc = dev.reaches(work, kCall, "work")) return rc;
   p.a = (const uint8_t *) a; p.b = (const uint8_t *) b; p.sa = sa; p.sb = sb;
   p.lda = lda; p.ldb = ldb; p.ldsa = ldsa; p.ldsb = ldsb;
   p.a_shift = ga == 128 ? 7 : 0; p.b_shift = gb == 128 ? 7 : 0;
   p.part = (float *) work;
   hipError_t e;
-  if (a_type == BOF_E4M3) e = b_type == BOF_E4M3 ? launch_product<BOF_E4M3, BOF_E4M3>(p, parts, (hipStream_t) stream) : launch_product<BOF_E4M3, BOF_E5M2>(p, parts, (hipStream_t) stream);
-  else e = b_type == BOF_E4M3 ? launch_product<BOF_E5M2, BOF_E4M3>(p, parts, (hipStream_t) stream) : launch_product<BOF_E5M2, BOF_E5M2>(p, parts, (hipStream_t) stream);
+  if (a_type == BOF_E4M3) e = b_type == BOF_E4M3 ? launch_product<BOF_E4M3, BOF_E4M3>(p, plan, (hipStream_t) stream) : launch_product<BOF_E4M3, BOF_E5M2>(p, plan, (hipStream_t) stream);
+  else e = b_type == BOF_E4M3 ? launch_product<BOF_E5M2, BOF_E4M3>(p, plan, (hipStream_t) stream) : launch_product<BOF_E5M2, BOF_E5M2>(p, plan, (hipStream_t) stream);
   BOF_HIP_TRY(e);
   return BOF_OK;
 }

@@ -138,7 +138,8 @@ def test_product_without_k(dev, c_type):
     assert torch.equal(c, torch.zeros_like(c))
 
 
-@pytest.mark.parametrize("m,n,k", [(2048, 2048, 512), (2048, 2304, 1024), (2100, 2300, 1100), (4000, 1300, 640), (2111, 2048, 1920), (2500, 2056, 2047), (4096, 4100, 256)])
+@pytest.mark.parametrize("m,n,k", [(2048, 2048, 512), (2048, 2304, 1024), (2100, 2300, 1100), (4000, 1300, 640), (2111, 2048, 1920), (2500, 2056, 2047), (4096, 4100, 256), (2048, 2050, 6500),
+                                   (3000, 3700, 1100), (3001, 3703, 640), (2999, 3750, 6500), (1500, 1500, 385), (1501, 1400, 4500)])
 @pytest.mark.parametrize("a,ga,b,gb", [("e4m3", 1, "e4m3", 128), ("e5m2", 1, "e4m3", 1), ("e4m3", 128, "e5m2", 1), ("e5m2", 128, "e5m2", 128)])
 def test_product_many_tiles(dev, m, n, k, a, ga, b, gb):
     """Outputs of many tiles, with whole and cut tiles at the edges, odd numbers of blocks and a short last one."""
@@ -147,16 +148,18 @@ def test_product_many_tiles(dev, m, n, k, a, ga, b, gb):
     A, B = Mat(g, m, k, a, ga, ld=up), Mat(g, n, k, b, gb, ld=up, lds=-(-k // 128) + 3)
     check_product(A, B, "bf16")
     check_product(Mat(g, m, k, a, ga, ld=k + 1), B, "bf16")
+    check_product(Mat(g, m, k, a, ga, ld=up + 4, offset=8), B, "bf16")
     check_product(A, B, "f16", alpha=0.5, beta=1.0, ldc=n + 1)
     check_product(A, B, "f32", beta=1.0)
 
 
-@pytest.mark.parametrize("m,n,k", [(128, 128, 129), (300, 400, 300), (333, 129, 6000), (130, 200, 12345), (256, 257, 4096), (700, 1030, 385)])
-@pytest.mark.parametrize("pad", [0, 1, 16])
+@pytest.mark.parametrize("m,n,k", [(128, 128, 129), (300, 400, 300), (333, 129, 6000), (130, 200, 12345), (256, 257, 4096), (700, 1030, 385), (100, 300, 2500), (127, 64, 5000),
+                                   (400, 2900, 8200)])
+@pytest.mark.parametrize("pad", [0, 1, 4, 16])
 def test_product_few_tiles(dev, m, n, k, pad):
     """Outputs of some tiles of 128, rows aligned or not, whole or split along k, with and without a short last block."""
     g = gen(m + k)
-    up = -(-k // 16) * 16 if pad == 16 else k + pad
+    up = -(-k // pad) * pad if pad > 1 else k + pad
     A, B = Mat(g, m, k, ld=up), Mat(g, n, k, "e5m2", 128, ld=up)
     for c_type in ("bf16", "f16", "f32"):
         check_product(A, B, c_type, alpha=-0.5, beta=0.25, ldc=n + 3)
