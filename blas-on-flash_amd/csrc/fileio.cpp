@@ -365,6 +365,9 @@ static int rw_full(int fd, bool wr, char *buf, uint64_t len, uint64_t off) {
   return 0;
 }
 
+// A buffer the kernel cannot pin -- the pinned memory of some machines is a mapping of the GPU driver's without pages of its
+// own -- makes every O_DIRECT request of it end in EFAULT: such a request goes through the buffered twin, which copies (and
+// still reports EFAULT for an address that is none).
 static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_t n_strides,
                       uint64_t len, void *buf, bool use_aio) {
   if (n_strides == 0 || len == 0) return 0;
@@ -390,7 +393,7 @@ static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_
       for (uint64_t o = 0; o < len; o += piece)
         pieces.push_back(IoPiece{fd, wr, p + s * len + o, std::min(piece, len - o), offset + s * stride + o});
     const int rc = uring_run(pieces);
-    if (rc != -ENOSYS) {
+    if (rc != -ENOSYS && rc != -EFAULT) {
       (wr ? g_wr_ops : g_rd_ops) += pieces.size();
       return rc;
     }
@@ -412,13 +415,17 @@ static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_
       }
     }
     const int rc = aio_run(cbs);
-    if (rc != -ENOSYS) {
+    if (rc != -ENOSYS && rc != -EFAULT) {
       (wr ? g_wr_ops : g_rd_ops) += cbs.size();
       return rc;
     }
   }
   for (uint64_t s = 0; s < n_strides; s++) {
-    const int rc = rw_full(fd, wr, p + s * len, len, offset + s * stride);
+    int rc = rw_full(fd, wr, p + s * len, len, offset + s * stride);
+    if (rc == -EFAULT && direct && aligned) {
+      const int twin = buffered_twin(fd);
+      rc = twin < 0 ? -EBADF : rw_full(twin, wr, p + s * len, len, offset + s * stride);
+    }
     if (rc) return rc;
   }
   return 0;
