@@ -1084,6 +1084,7 @@ Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, int max
   double least = 1e30;
   auto consider = [&](Kind kind, int tm, int tn, double one, double two) {
     const int64_t tiles = ((m + tm - 1) / tm) * ((n + tn - 1) / tn);
+    if (tiles >= (1 << 23)) return;   // (512 threads each: a launch holds less than 2^32)
     for (int64_t parts = 1; parts <= max_parts && (parts == 1 || (parts * tiles <= (two > 0 ? 512 : 256) && parts * 8 <= nb + 7)); parts++) {
       const int64_t all = tiles * parts, rest = all % 512;
       const double rounds = two > 0 ? (double) (all / 512) * two + (rest == 0 ? 0 : rest <= 256 ? one : two) : (double) ((all + 255) / 256) * one;

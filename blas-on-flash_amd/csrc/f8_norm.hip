@@ -122,6 +122,13 @@ hipError_t launch_quant(const Quant &p, int group, hipStream_t st) {
   return hipGetLastError();
 }
 
+// A launch holds less than 2^32 threads along a dimension of its grid: workgroups go on along the second one.
+__device__ __forceinline__ int64_t workgroup() { return (int64_t) blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 grid_of(int64_t workgroups) {
+  const int64_t x = workgroups < (1 << 21) ? workgroups : 1 << 21;
+  return dim3((unsigned) x, (unsigned) ((workgroups + x - 1) / x));
+}
+
 // ---- a row and its team -------------------------------------------------------------
 // TEAM threads (a wave, or a workgroup of several) work on one row; thread t of the team holds CH chunks of eight
 // neighbours, chunk i at column (i * TEAM + t) * 8: 16 neighbouring lanes hold one block of 128.  Rows of up to
@@ -159,8 +166,8 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_kernel(Norm p) {
   constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
   __shared__ float part[TEAM < 256 ? 1 : TEAM / 64];
   const int t = threadIdx.x % TEAM;
-  const int64_t row = (int64_t) blockIdx.x * TEAMS + threadIdx.x / TEAM;
-  if (TEAMS > 1 && row >= p.rows) return;
+  const int64_t row = workgroup() * TEAMS + threadIdx.x / TEAM;
+  if (row >= p.rows) return;
   float h[CH][8];
   auto fetch = [&](int64_t c0) {
     Eight<T> x[CH], r[CH];
@@ -213,7 +220,7 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_kernel(Norm p) {
 template <int T, int TEAM, int CH, bool KEEP = true>
 void start_norm(const Norm &p, hipStream_t st) {
   constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
-  norm_kernel<T, TEAM, CH, KEEP><<<(unsigned) ((p.rows + TEAMS - 1) / TEAMS), TEAM < 256 ? 256 : TEAM, 0, st>>>(p);
+  norm_kernel<T, TEAM, CH, KEEP><<<grid_of((p.rows + TEAMS - 1) / TEAMS), TEAM < 256 ? 256 : TEAM, 0, st>>>(p);
 }
 template <int T>
 hipError_t launch_norm(const Norm &p, hipStream_t st) {
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_grad_kernel(Norm
 __global__ void __launch_bounds__(256) norm_grad_join_kernel(const float *part, int teams, int64_t n, float beta, float *dw) {
   __shared__ f32x4 sums[32][8];
   const int t = threadIdx.x, col = t & 7, slice = t >> 3;
-  const int64_t np = part_columns(n), c = (int64_t) blockIdx.x * 32 + col * 4;
+  const int64_t np = part_columns(n), c = workgroup() * 32 + col * 4;
   const int per = (teams + 31) / 32, g0 = slice * per, g1 = min(teams, g0 + per);
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   if (c < n) {
@@ -329,7 +336,7 @@ __global__ void __launch_bounds__(256) norm_grad_join_kernel(const float *part, 
   sums[slice][col] = sum;
   __syncthreads();
   if (t >= 64) return;
-  const int64_t to = (int64_t) blockIdx.x * 32 + (t & 31);
+  const int64_t to = workgroup() * 32 + (t & 31);
   float v = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; i++) v += sums[(t >> 5) * 16 + i][(t & 31) >> 2][t & 3];
@@ -358,7 +365,7 @@ hipError_t launch_norm_grad(const NormGrad &p, hipStream_t st) {
   else if (p.n <= team_width(256, 4)) start_norm_grad<T, 256, 4>(p, st);
   else if (p.n <= team_width(1024, 2)) start_norm_grad<T, 1024, 2>(p, st);
   else start_norm_grad<T, 1024, 1, false>(p, st);
-  if (p.dw) norm_grad_join_kernel<<<(unsigned) ((p.n + 31) / 32), 256, 0, st>>>(p.part, p.teams, p.n, p.beta, p.dw);
+  if (p.dw) norm_grad_join_kernel<<<grid_of((p.n + 31) / 32), 256, 0, st>>>(p.part, p.teams, p.n, p.beta, p.dw);
   return hipGetLastError();
 }
 
@@ -452,7 +459,7 @@ int bof_rmsnorm_grad(int64_t rows, int64_t n, int type, const void *dy, int64_t 
   if (int rc = dw ? dev.reaches(dw, kCall, "dw") : 0) return rc;
   if (rows == 0) {   // no rows: dw = beta * dw
     drop_stale_error();
-    norm_grad_join_kernel<<<(unsigned) ((n + 31) / 32), 256, 0, hs>>>(nullptr, 0, n, beta, dw);
+    norm_grad_join_kernel<<<grid_of((n + 31) / 32), 256, 0, hs>>>(nullptr, 0, n, beta, dw);
     BOF_HIP_TRY(hipGetLastError());
     return BOF_OK;
   }

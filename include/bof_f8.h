@@ -17,7 +17,7 @@
  *
  * Conventions: every pointer is device memory (or host memory that the device maps) of the stream's device -- a
  * pointer to anything else is refused; no alignment is asked for beyond that of the element type (rows that begin at
- * multiples of 16 bytes are faster); outputs must not overlap inputs unless said otherwise; bytes between the rows
+ * multiples of 4 bytes are faster, those that begin at multiples of 128 fastest); outputs must not overlap inputs unless said otherwise; bytes between the rows
  * and behind the last one are left as they were.  All calls are asynchronous on `stream`, allocate nothing, keep
  * nothing and may be captured into a graph: scratch memory is the caller's `work`, which no two calls that may run at
  * the same time may share.  Errors as in bof_hip.h (BOF_EINVAL and bof_last_error()); an empty result is BOF_OK.

@@ -657,6 +657,41 @@ def test_a_captured_step_replays(dev):
         assert torch.equal(a, b)
 
 
+def enough_memory(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of device memory")
+
+
+def test_norm_of_more_rows_than_a_grid_dimension_holds(dev):
+    """2^22 rows of a workgroup of 1024 threads each are 2^32 threads."""
+    enough_memory(70)
+    rows, n = (1 << 22) + 5, 8200
+    x = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    x[:2], x[-7:] = 0.5, 2.0
+    w = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    rstd = torch.full((rows + 3,), 7.0, device="cuda")
+    bofhip.rmsnorm_f8(rows, n, bofhip.BF16, at(x), n, 0, 0, at(w), 0.0, 0, 0, bofhip.E4M3, 0, 0, 0, 0, rstd=at(rstd), stream=stream())
+    torch.cuda.synchronize()
+    assert rstd[:2].tolist() == [2.0, 2.0] and rstd[rows - 7:].tolist() == [0.5] * 7 + [7.0] * 3
+
+
+def test_gradient_of_a_row_longer_than_a_grid_dimension_holds(dev):
+    """2^29 columns are 2^32 threads of the join."""
+    enough_memory(12)
+    n = (1 << 29) + 40
+    h = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    dy, dx, rstd = torch.zeros_like(h), torch.empty_like(h), torch.full((1,), 0.5, device="cuda")
+    places = torch.tensor([0, 31, 5000, (1 << 29) - 1, 1 << 29, n - 1], device="cuda")
+    dy[places] = torch.arange(1, 7, device="cuda").bfloat16()
+    dw = torch.full((n + 8,), 9.0, device="cuda")
+    work = torch.empty(bofhip.rmsnorm_grad_workspace_bytes(1, n), dtype=torch.uint8, device="cuda")
+    bofhip.rmsnorm_grad(1, n, bofhip.BF16, at(dy), n, at(h), n, at(h), at(rstd), 0, 0, at(dx), n, 0.0, at(dw), at(work), work.numel(), stream())
+    torch.cuda.synchronize()
+    assert torch.equal(dw[places], torch.arange(1, 7, device="cuda") * 0.5)
+    assert dw[:n].count_nonzero() == 6 and torch.equal(dw[n:], torch.full((8,), 9.0, device="cuda"))
+
+
 def test_two_streams_at_once(dev):
     """Two layers stepping on two streams, without waiting for one another, each with its own workspace."""
     layers = [Layer(64, 512, 512, seed=s) for s in (1, 2)]
