@@ -552,6 +552,7 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
 // 1024 x 4096 x 4096 in 19 us for 28.
 // 128 x 160: the same, for outputs that it covers in fewer rounds of 256 workgroups: 1021 x 5000 x 4100 without padding in 34.6 us for 53
 // (rows of 4100 bytes lie across the L2's lines and cost 5 of them, the short block 4).
+// 256 x 128, three blocks: for one round of what takes 128 x 128 two: 2048 x 4096 x 4096 in 32 us for 38.
 // 64 x 32, six blocks, two workgroups a CU, for few rows and few columns: bound by the bytes of B, 48 x 8192 x 4096 in 8.9 us
 // (3.8 TB/s), 4.8 TB/s at 8 x 8192 x 8192; with eight blocks and one workgroup a CU 128 x 8192 x 4096 took 15.5 us for 12.3.
 template <int X_, int Y_, int WM_, int ST_, bool DMA>
@@ -561,6 +562,7 @@ struct Ring {
   static constexpr int B0 = 8 * TM, BLOCK = B0 + 8 * TN, S0 = ST * BLOCK;        // chunks of 16 bytes: B rows, a block, where the scales begin
   static constexpr int ROWS = TM + TN, CHUNKS = S0 + scale_chunks(ROWS);
   static constexpr int PA = TM / 32, PIECES = PA + TN / 32;                      // of 32 rows (8 a wave), A's, then B's
+  static constexpr int STEPS = ST % 2 ? 2 * ST : ST;                             // until place in the ring and set of fragments come round
   u32x4 *lds;
   uint32_t voff[PIECES];         // of this thread's row and chunk
   uint32_t to;                   // LDS address of this wave's part of a piece in block 0 (DMA)
@@ -570,23 +572,23 @@ struct Ring {
   u32x4 staged[2][DMA ? 1 : PIECES];
 };
 
-// Step t, U = its place in the ring; a, b: where the block to fetch begins; sc: the scale byte of block t + 1.
+// Step t, U = t mod STEPS; a, b: where the block to fetch begins; sc: the scale byte of block t + 1.
 template <int TA, int TB, bool DMA, int U, class S, int X, int Y>
 __device__ __forceinline__ void ring_step(S &s, uint64_t a, uint64_t b, int sc, Frag<false> (&fa)[2][X], Frag<false> (&fb)[2][Y], f32x4 (&acc)[X][Y]) {
-  constexpr int P = U & 1, N = X * Y, LAST = N - N / 5, WORK = 2 * S::PIECES;   // MFMAs, those in front of the barrier, work beside them
+  constexpr int P = U & 1, AT = U % S::ST, N = X * Y, LAST = N - N / 5, WORK = 2 * S::PIECES;   // MFMAs, those in front of the barrier, work beside them
   static_assert(X + Y == S::PIECES, "a fragment to read for every piece");
   auto piece = [&](int q) {
     const uint64_t from = q < S::PA ? a : b;
     if constexpr (DMA) {
-      dma16(s.voff[q], from, s.to + U * S::BLOCK * 16 + q * 4096);
+      dma16(s.voff[q], from, s.to + AT * S::BLOCK * 16 + q * 4096);
     } else {
       u32x4 &v = s.staged[P][q];
-      s.lds[s.put + (U + 3) % S::ST * S::BLOCK + q * 256] = v;
+      s.lds[s.put + (AT + 3) % S::ST * S::BLOCK + q * 256] = v;
       __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(from) + s.voff[q], 16);
     }
   };
   auto read = [&](int f) {   // fragment f of the next block
-    const u32x4 *block = s.lds + (U + 1) % S::ST * S::BLOCK;
+    const u32x4 *block = s.lds + (AT + 1) % S::ST * S::BLOCK;
     if (f < Y) {
       fb[P ^ 1][f].q = both(block[s.b_lo + f * 128], block[s.b_hi + f * 128]);
       fb[P ^ 1][f].s = s.sb[sc + f * 320];
@@ -620,7 +622,7 @@ template <class F, int... U>
 __device__ __forceinline__ void each_place(F &&f, std::integer_sequence<int, U...>) { (f(std::integral_constant<int, U>()), ...); }
 
 template <int TA, int TB, int X, int Y, int WM, int ST, bool DMA>
-__global__ void __launch_bounds__(256, X == 4 ? 1 : 2) f8_ring_kernel(F8Product q, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(256, X >= 4 ? 1 : 2) f8_ring_kernel(F8Product q, int tiles_m, int tiles_n) {
   using S = Ring<X, Y, WM, ST, DMA>;
   __shared__ u32x4 lds[S::CHUNKS];
   const F8Product p = part_of(q, blockIdx.y);
@@ -724,12 +726,12 @@ __global__ void __launch_bounds__(256, X == 4 ? 1 : 2) f8_ring_kernel(F8Product 
     if constexpr (S::ROWS > 256) w = next_scales(s_row2, seg * 16 + 16, nb);
     put_half(seg + 1, v, w);
   };
-  while (kb + ST <= full) {
+  while (kb + S::STEPS <= full) {
     more_scales();
-    each_place(next, std::make_integer_sequence<int, ST>());
+    each_place(next, std::make_integer_sequence<int, S::STEPS>());
   }
   more_scales();
-  each_place([&](auto place) { if (kb < full) next(place); }, std::make_integer_sequence<int, ST - 1>());
+  each_place([&](auto place) { if (kb < full) next(place); }, std::make_integer_sequence<int, S::STEPS - 1>());
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   if (tail) {   // the short block: through registers, zeros behind k
@@ -1058,7 +1060,7 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
 }
 
 // ---- which kernel --------------------------------------------------------------------
-enum Kind { kAny, kRows, kRing64, kRing128, kRing160, kTile256, kWide128, kWide256 };
+enum Kind { kAny, kRows, kRing64, kRing128, kRing160, kRing256, kTile256, kWide128, kWide256 };
 struct Plan {
   Kind kind;
   int parts;   // along k
@@ -1070,12 +1072,13 @@ constexpr int kMaxParts = 32;
 //   64 x 32      one workgroup a CU 0.16, two 0.30     48 x 8192 x 4096 9 us, 128 x 8192 x 4096 12 (128 x 128: 14 and 17)
 //   128 x 128    0.50                                  1024 x 4096 x 4096 20 us (64 x 32: 40, 256 x 256: 45)
 //   128 x 160    0.64                                  1024 x 5120 x 4096 24 us (128 x 128: 34, 256 x 256: 46)
+//   256 x 128    0.85                                  2048 x 4096 x 4096 32 us (128 x 128: 38, 256 x 256: 46); only by DMA: staged it spills
 //   256 x 256    1.35                                  4096 x 4096 x 4096 56 us (128 x 128: 76)
 //   wide         0.9 (128 x 128), 1.7 (256 x 128)
 // One to sixteen rows of A and a workgroup a CU at most go to the kernel for few rows: 1 x 4096 x 4096 in 5.9 us, in 7.5 by tiles
 // of 64 x 32; 8 x 4096 x 8192 in 10.8 and 11.1; 1 x 8192 x 4096 in 8.8 and 8.4, 1 x 512 x 16384 in 11.9 and 9.0.  Wide: all up to
 // 32 rows, 32 x 4096 x 4096 in 12.0 us (33 rows by tiles: 15.6).
-Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, int max_parts) {
+Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, bool dma, int max_parts) {
   if (m <= 16 && n <= 4096 && k <= 8192 && near) return {kRows, 1};
   if (wide && m <= 32 && n <= (1 << 26) && near) return {kRows, 1};
   if (k < 128 || !near) return {kAny, 1};
@@ -1099,6 +1102,7 @@ Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, int max
     consider(kRing64, 64, 32, 0.16, 0.30);
     consider(kRing128, 128, 128, 0.50, 0);
     consider(kRing160, 128, 160, 0.64, 0);
+    if (dma) consider(kRing256, 256, 128, 0.85, 0);
     if (m >= 256 && n >= 256) max_parts = 1, consider(kTile256, 256, 256, 1.35, 0);
   }
   return best;
@@ -1106,14 +1110,14 @@ Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, int max
 
 // what the DMA to LDS needs of a row: 16-byte chunks at multiples of four bytes (at no loss: reads from the L2 run at 20 TB/s at any
 // such address, at 10 at odd ones)
-bool rows_aligned(const F8Product &p) {
-  return p.lda % 4 == 0 && p.ldb % 4 == 0 && reinterpret_cast<uintptr_t>(p.a) % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % 4 == 0;
+bool rows_aligned(const void *a, int64_t lda, const void *b, int64_t ldb) {
+  return lda % 4 == 0 && ldb % 4 == 0 && reinterpret_cast<uintptr_t>(a) % 4 == 0 && reinterpret_cast<uintptr_t>(b) % 4 == 0;
 }
 
 template <int TA, int TB>
 void start_tiles(const F8Product &p, hipStream_t st) {
   const int tiles_m = (p.m + 255) / 256, tiles_n = (p.n + 255) / 256;
-  if (rows_aligned(p)) f8_tile_kernel<TA, TB, 8, 8, true><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
+  if (rows_aligned(p.a, p.lda, p.b, p.ldb)) f8_tile_kernel<TA, TB, 8, 8, true><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
   else f8_tile_kernel<TA, TB, 8, 8, false><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 template <int TA, int TB, int X, int Y, int WM, int ST>
@@ -1121,7 +1125,7 @@ void start_ring(const F8Product &p, int parts, hipStream_t st) {
   using S = Ring<X, Y, WM, ST, true>;
   const int tiles_m = (p.m + S::TM - 1) / S::TM, tiles_n = (p.n + S::TN - 1) / S::TN;
   const dim3 grid((unsigned) (tiles_m * tiles_n), (unsigned) parts);
-  if (rows_aligned(p)) f8_ring_kernel<TA, TB, X, Y, WM, ST, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
+  if (rows_aligned(p.a, p.lda, p.b, p.ldb)) f8_ring_kernel<TA, TB, X, Y, WM, ST, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
   else f8_ring_kernel<TA, TB, X, Y, WM, ST, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 
@@ -1129,7 +1133,7 @@ template <int TA, int TB, int X>
 void start_wide(const F8Product &p, int parts, hipStream_t st) {
   const int tiles_m = (p.m + 32 * X - 1) / (32 * X), tiles_n = (p.n + 127) / 128;
   const dim3 grid((unsigned) (tiles_m * tiles_n), (unsigned) parts);
-  if (rows_aligned(p)) f8_wide_kernel<TA, TB, X, true><<<grid, 512, 0, st>>>(p, tiles_m, tiles_n);
+  if (rows_aligned(p.a, p.lda, p.b, p.ldb)) f8_wide_kernel<TA, TB, X, true><<<grid, 512, 0, st>>>(p, tiles_m, tiles_n);
   else f8_wide_kernel<TA, TB, X, false><<<grid, 512, 0, st>>>(p, tiles_m, tiles_n);
 }
 
@@ -1162,6 +1166,12 @@ hipError_t launch_product(F8Product p, Plan plan, hipStream_t st) {
       break;
     case kRing64: start_ring<TA, TB, 2, 1, 2, 6>(p, parts, st); break;
     case kRing128: start_ring<TA, TB, 4, 4, 2, 4>(p, parts, st); break;
+    case kRing256: {
+      using S = Ring<8, 4, 2, 3, true>;
+      const int tiles_m = (p.m + S::TM - 1) / S::TM, tiles_n = (p.n + S::TN - 1) / S::TN;
+      f8_ring_kernel<TA, TB, 8, 4, 2, 3, true><<<dim3((unsigned) (tiles_m * tiles_n), (unsigned) parts), 256, 0, st>>>(p, tiles_m, tiles_n);
+      break;
+    }
     case kRing160: start_ring<TA, TB, 4, 5, 2, 4>(p, parts, st); break;
     case kTile256: start_tiles<TA, TB>(p, st); break;
     case kWide128: start_wide<TA, TB, 4>(p, parts, st); break;
@@ -1184,8 +1194,8 @@ extern "C" {
 
 uint64_t bof_f8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0 || m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return 0;
-  const int narrow = plan_product(m, n, k, false, true, kMaxParts).parts, wide = plan_product(m, n, k, true, true, kMaxParts).parts;
-  const int parts = narrow > wide ? narrow : wide;
+  int parts = plan_product(m, n, k, true, true, true, kMaxParts).parts;
+  for (bool dma : {false, true}) parts = std::max(parts, plan_product(m, n, k, false, true, dma, kMaxParts).parts);
   return parts > 1 ? (uint64_t) parts * (uint64_t) m * (uint64_t) n * 4u : 0;
 }
 
@@ -1223,7 +1233,7 @@ int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int
     if (int rc = dev.reaches(q, kCall, name)) return rc;
   const uint64_t room = work ? work_bytes / ((uint64_t) m * (uint64_t) n * 4u) : 0;
   const bool near = lda <= (1 << 24) && ldb <= (1 << 24) && ldsa <= (1 << 24) && ldsb <= (1 << 24);   // a tile of 256 rows: offsets of 32 bits
-  const Plan plan = plan_product(m, n, k, c_type == BOF_F32, near, room < 2 ? 1 : room < kMaxParts ? (int) room : kMaxParts);
+  const Plan plan = plan_product(m, n, k, c_type == BOF_F32, near, rows_aligned(a, lda, b, ldb), room < 2 ? 1 : room < kMaxParts ? (int) room : kMaxParts);
   if (plan.parts > 1)
     if (int rc = dev.reaches(work, kCall, "work")) return rc;
   p.a = (const uint8_t *) a; p.b = (const uint8_t *) b; p.sa = sa; p.sb = sb;
