@@ -1220,7 +1220,8 @@ int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int
   if (int rc = dev.reaches(c, kCall, "C")) return rc;
   F8Product p{};
   p.ldc = ldc; p.m = (int) m; p.n = (int) n; p.k = product ? (int) k : 0;
-  p.alpha = alpha; p.beta = beta; p.c = c; p.c_type = c_type;
+  p.alpha = product ? alpha : 0.f; p.beta = beta;   // (no product: beta * C whatever alpha is)
+  p.c = c; p.c_type = c_type;
   if (!product) {
     if (beta == 1.f) return BOF_OK;
     const int64_t wg = (m * n + 255) / 256;

@@ -138,6 +138,32 @@ def test_product_without_k(dev, c_type):
     assert torch.equal(c, torch.zeros_like(c))
 
 
+@pytest.mark.parametrize("alpha", [float("inf"), float("nan")])
+def test_product_without_k_and_any_alpha(dev, alpha):
+    c = torch.randn(5, 8, device="cuda")
+    c0 = c.clone()
+    bofhip.f8_gemm(5, 8, 0, alpha, 0, 0, bofhip.E4M3, 0, 0, 1, 0, 0, bofhip.E4M3, 0, 0, 1, -3.0, at(c), 8, bofhip.F32, 0, 0, stream())
+    assert torch.equal(c, c0 * -3)
+
+
+@pytest.mark.parametrize("m,n,k,c_type", [(3, 300, 500, "bf16"), (40, 200, 300, "f16"), (300, 1000, 700, "bf16"), (7, 90, 300, "f32"), (100, 300, 400, "f32")])
+def test_product_of_mapped_host_memory(dev, m, n, k, c_type):
+    g = gen(k)
+    A, B = Mat(g, m, k, ld=k), Mat(g, n, k, group=128, ld=k)
+    want = check_product(A, B, c_type)
+    for x in (A, B):
+        x.q = torch.empty(x.q.shape, dtype=torch.uint8, pin_memory=True).copy_(x.q)
+        x.s = torch.empty(x.s.shape, dtype=torch.uint8, pin_memory=True).copy_(x.s)
+    c = torch.zeros_like(want)
+    product(A, B, c, c_type)
+    torch.cuda.synchronize()
+    ref = torch.zeros_like(want)
+    for x in (A, B):
+        x.q, x.s = x.q.cuda(), x.s.cuda()
+    product(A, B, ref, c_type)
+    assert torch.equal(c, ref)
+
+
 @pytest.mark.parametrize("m,n,k", [(2048, 2048, 512), (2048, 2304, 1024), (2100, 2300, 1100), (4000, 1300, 640), (2111, 2048, 1920), (2500, 2056, 2047), (4096, 4100, 256), (2048, 2050, 6500),
                                    (3000, 3700, 1100), (3001, 3703, 640), (2999, 3750, 6500), (1500, 1500, 385), (1501, 1400, 4500),
                                    (1600, 4000, 700), (1601, 4096, 1281), (1800, 4001, 5000)])
