@@ -550,7 +550,9 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
 // 128 x 128, four blocks, one workgroup a CU: a block takes 0.5 us of it, two thirds of that LDS (64 KB of fragments are read
 // for 32 KB of rows, at 128 bytes a cycle); two images of LDS and two workgroups a CU took 0.8 us on an idle card:
 // 1024 x 4096 x 4096 in 19 us for 28.
-// 128 x 160: the same, for outputs that it covers in fewer rounds of 256 workgroups: 1021 x 5000 x 4100 without padding in 34.6 us for 53
+// Two of 128 x 128 a CU with two blocks each: slower in its steps, which wait for their fetches, but one loads and stores
+// while the other multiplies: for many tiles and few blocks.
+// 128 x 160: the same as the first, for outputs that it covers in fewer rounds of 256 workgroups: 1021 x 5000 x 4100 without padding in 34.6 us for 53
 // (rows of 4100 bytes lie across the L2's lines and cost 5 of them, the short block 4).
 // 256 x 128, three blocks: for one round of what takes 128 x 128 two: 2048 x 4096 x 4096 in 32 us for 38.
 // 64 x 32, six blocks, two workgroups a CU, for few rows and few columns: bound by the bytes of B, 48 x 8192 x 4096 in 8.9 us
@@ -622,7 +624,7 @@ template <class F, int... U>
 __device__ __forceinline__ void each_place(F &&f, std::integer_sequence<int, U...>) { (f(std::integral_constant<int, U>()), ...); }
 
 template <int TA, int TB, int X, int Y, int WM, int ST, bool DMA>
-__global__ void __launch_bounds__(256, X >= 4 ? 1 : 2) f8_ring_kernel(F8Product q, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(256, X >= 4 && ST > 2 ? 1 : 2) f8_ring_kernel(F8Product q, int tiles_m, int tiles_n) {
   using S = Ring<X, Y, WM, ST, DMA>;
   __shared__ u32x4 lds[S::CHUNKS];
   const F8Product p = part_of(q, blockIdx.y);
@@ -1060,21 +1062,24 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, int parts) {
 }
 
 // ---- which kernel --------------------------------------------------------------------
-enum Kind { kAny, kRows, kRing64, kRing128, kRing160, kRing256, kTile256, kWide128, kWide256 };
+enum Kind { kAny, kRows, kRing64, kRing128, kTwo128, kRing160, kRing256, kTile256, kWide128, kWide256 };
 struct Plan {
   Kind kind;
   int parts;   // along k
 };
 constexpr int kMaxParts = 32;
 
-// The kernel, and the parts along k, of least time by this estimate: us that a block of k takes a CU that holds one workgroup, the
-// same for two of them (0: it holds one), and 3 us; for parts a join of 4 us and 4 TB/s for what they write and it reads.
-//   64 x 32      one workgroup a CU 0.16, two 0.30     48 x 8192 x 4096 9 us, 128 x 8192 x 4096 12 (128 x 128: 14 and 17)
-//   128 x 128    0.50                                  1024 x 4096 x 4096 20 us (64 x 32: 40, 256 x 256: 45)
-//   128 x 160    0.64                                  1024 x 5120 x 4096 24 us (128 x 128: 34, 256 x 256: 46)
-//   256 x 128    0.85                                  2048 x 4096 x 4096 32 us (128 x 128: 38, 256 x 256: 46); only by DMA: staged it spills
-//   256 x 256    1.35                                  4096 x 4096 x 4096 56 us (128 x 128: 76)
-//   wide         0.9 (128 x 128), 1.7 (256 x 128)
+// The kernel, and the parts along k, of least time by this estimate, in us: 1, and for every round of workgroups what it takes to
+// begin and to store, and what a block of k takes; a round is one workgroup a CU, or two where two numbers stand (the second
+// is for two).  For parts a join of 4 us and 4 TB/s for what they write and it reads.
+//                 round      block
+//   64 x 32       3.0, 3.2   0.16, 0.30   48 x 8192 x 4096 9 us, 128 x 8192 x 4096 12 (128 x 128: 14 and 17)
+//   128 x 128     5.0        0.48         1024 x 4096 x 4096 20 us (64 x 32: 40, 256 x 256: 45)
+//     two a CU    4.5, 6.0   0.55, 1.00   12416 x 4669 x 256 59 us (256 x 256: 72), 2048 x 4096 x 1024 16 (256 x 128: 17); only by DMA
+//   128 x 160     8.0        0.45         1024 x 5120 x 4096 24 us (128 x 128: 34, 256 x 256: 46)
+//   256 x 128     9.5        0.75         2048 x 4096 x 4096 33 us (128 x 128: 38, 256 x 256: 46); only by DMA: staged it spills
+//   256 x 256     13         1.30         4096 x 4096 x 4096 55 us (128 x 128: 76), 8192 x 8192 x 1024 103 (two of 128 x 128: 111)
+//   wide          3.0        0.9 (128 x 128), 1.7 (256 x 128)
 // One to sixteen rows of A and a workgroup a CU at most go to the kernel for few rows: 1 x 4096 x 4096 in 5.9 us, in 7.5 by tiles
 // of 64 x 32; 8 x 4096 x 8192 in 10.8 and 11.1; 1 x 8192 x 4096 in 8.8 and 8.4, 1 x 512 x 16384 in 11.9 and 9.0.  Wide: all up to
 // 32 rows, 32 x 4096 x 4096 in 12.0 us (33 rows by tiles: 15.6).
@@ -1085,25 +1090,32 @@ Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, bool dm
   const int64_t nb = k / 128;
   Plan best{kAny, 1};
   double least = 1e30;
-  auto consider = [&](Kind kind, int tm, int tn, double one, double two) {
+  struct Cost { double round, block; };
+  auto consider = [&](Kind kind, int tm, int tn, Cost one, Cost two) {   // two.round 0: a CU holds one workgroup
     const int64_t tiles = ((m + tm - 1) / tm) * ((n + tn - 1) / tn);
     if (tiles >= (1 << 23)) return;   // (512 threads each: a launch holds less than 2^32)
-    for (int64_t parts = 1; parts <= max_parts && (parts == 1 || (parts * tiles <= (two > 0 ? 512 : 256) && parts * 8 <= nb + 7)); parts++) {
-      const int64_t all = tiles * parts, rest = all % 512;
-      const double rounds = two > 0 ? (double) (all / 512) * two + (rest == 0 ? 0 : rest <= 256 ? one : two) : (double) ((all + 255) / 256) * one;
-      const double us = (double) ((nb + parts - 1) / parts) * rounds + 3 + (parts > 1 ? 4 + (double) parts * (double) m * (double) n * 8 / 4e6 : 0);
+    const int64_t full = two.round > 0 ? 512 : 256;
+    for (int64_t parts = 1; parts <= max_parts && (parts == 1 || (parts * tiles <= full && parts * 8 <= nb + 7)); parts++) {
+      const int64_t all = tiles * parts, rest = all % full;
+      const double blocks = (double) ((nb + parts - 1) / parts);
+      auto round = [&](Cost c) { return c.round + blocks * c.block; };
+      const double us = 1 + (double) (all / full) * round(full == 512 ? two : one) + (rest == 0 ? 0 : rest <= 256 ? round(one) : round(two)) +
+                        (parts > 1 ? 4 + (double) parts * (double) m * (double) n * 8 / 4e6 : 0);
       if (us < least) { least = us; best = {kind, (int) parts}; }
     }
   };
   if (wide) {
-    consider(kWide128, 128, 128, 0.9, 0);
-    if (m >= 256 && n >= 128) consider(kWide256, 256, 128, 1.7, 0);
+    consider(kWide128, 128, 128, {3, 0.9}, {0, 0});
+    if (m >= 256 && n >= 128) consider(kWide256, 256, 128, {3, 1.7}, {0, 0});
   } else {
-    consider(kRing64, 64, 32, 0.16, 0.30);
-    consider(kRing128, 128, 128, 0.50, 0);
-    consider(kRing160, 128, 160, 0.64, 0);
-    if (dma) consider(kRing256, 256, 128, 0.85, 0);
-    if (m >= 256 && n >= 256) max_parts = 1, consider(kTile256, 256, 256, 1.35, 0);
+    consider(kRing64, 64, 32, {3, 0.16}, {3.2, 0.30});
+    consider(kRing128, 128, 128, {5, 0.48}, {0, 0});
+    consider(kRing160, 128, 160, {8, 0.45}, {0, 0});
+    if (dma) {
+      consider(kTwo128, 128, 128, {4.5, 0.55}, {6, 1});
+      consider(kRing256, 256, 128, {9.5, 0.75}, {0, 0});
+    }
+    if (m >= 256 && n >= 256) max_parts = 1, consider(kTile256, 256, 256, {13, 1.3}, {0, 0});
   }
   return best;
 }
@@ -1120,13 +1132,13 @@ void start_tiles(const F8Product &p, hipStream_t st) {
   if (rows_aligned(p.a, p.lda, p.b, p.ldb)) f8_tile_kernel<TA, TB, 8, 8, true><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
   else f8_tile_kernel<TA, TB, 8, 8, false><<<(unsigned) (tiles_m * tiles_n), 256, 0, st>>>(p, tiles_m, tiles_n);
 }
-template <int TA, int TB, int X, int Y, int WM, int ST>
+template <int TA, int TB, int X, int Y, int WM, int ST, bool ANY = true>   // (ANY: also for rows that the DMA does not take)
 void start_ring(const F8Product &p, int parts, hipStream_t st) {
   using S = Ring<X, Y, WM, ST, true>;
   const int tiles_m = (p.m + S::TM - 1) / S::TM, tiles_n = (p.n + S::TN - 1) / S::TN;
   const dim3 grid((unsigned) (tiles_m * tiles_n), (unsigned) parts);
-  if (rows_aligned(p.a, p.lda, p.b, p.ldb)) f8_ring_kernel<TA, TB, X, Y, WM, ST, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
-  else f8_ring_kernel<TA, TB, X, Y, WM, ST, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
+  if (!ANY || rows_aligned(p.a, p.lda, p.b, p.ldb)) f8_ring_kernel<TA, TB, X, Y, WM, ST, true><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
+  else if constexpr (ANY) f8_ring_kernel<TA, TB, X, Y, WM, ST, false><<<grid, 256, 0, st>>>(p, tiles_m, tiles_n);
 }
 
 template <int TA, int TB, int X>
@@ -1166,12 +1178,8 @@ hipError_t launch_product(F8Product p, Plan plan, hipStream_t st) {
       break;
     case kRing64: start_ring<TA, TB, 2, 1, 2, 6>(p, parts, st); break;
     case kRing128: start_ring<TA, TB, 4, 4, 2, 4>(p, parts, st); break;
-    case kRing256: {
-      using S = Ring<8, 4, 2, 3, true>;
-      const int tiles_m = (p.m + S::TM - 1) / S::TM, tiles_n = (p.n + S::TN - 1) / S::TN;
-      f8_ring_kernel<TA, TB, 8, 4, 2, 3, true><<<dim3((unsigned) (tiles_m * tiles_n), (unsigned) parts), 256, 0, st>>>(p, tiles_m, tiles_n);
-      break;
-    }
+    case kTwo128: start_ring<TA, TB, 4, 4, 2, 2, false>(p, parts, st); break;
+    case kRing256: start_ring<TA, TB, 8, 4, 2, 3, false>(p, parts, st); break;
     case kRing160: start_ring<TA, TB, 4, 5, 2, 4>(p, parts, st); break;
     case kTile256: start_tiles<TA, TB>(p, st); break;
     case kWide128: start_wide<TA, TB, 4>(p, parts, st); break;

@@ -166,7 +166,7 @@ def test_product_of_mapped_host_memory(dev, m, n, k, c_type):
 
 @pytest.mark.parametrize("m,n,k", [(2048, 2048, 512), (2048, 2304, 1024), (2100, 2300, 1100), (4000, 1300, 640), (2111, 2048, 1920), (2500, 2056, 2047), (4096, 4100, 256), (2048, 2050, 6500),
                                    (3000, 3700, 1100), (3001, 3703, 640), (2999, 3750, 6500), (1500, 1500, 385), (1501, 1400, 4500),
-                                   (1600, 4000, 700), (1601, 4096, 1281), (1800, 4001, 5000)])
+                                   (1600, 4000, 700), (1601, 4096, 1281), (1800, 4001, 5000), (4096, 4000, 2100), (5000, 1000, 700)])
 @pytest.mark.parametrize("a,ga,b,gb", [("e4m3", 1, "e4m3", 128), ("e5m2", 1, "e4m3", 1), ("e4m3", 128, "e5m2", 1), ("e5m2", 128, "e5m2", 128)])
 def test_product_many_tiles(dev, m, n, k, a, ga, b, gb):
     """Outputs of many tiles, with whole and cut tiles at the edges, odd numbers of blocks and a short last one."""
