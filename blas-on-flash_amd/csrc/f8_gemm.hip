@@ -311,14 +311,21 @@ __device__ __forceinline__ i32x8 both(u32x4 lo, u32x4 hi) {
 }
 
 // The slab's product, its accumulators pinned to the accumulator half of the register file (left to itself the compiler moves
-// them through both: 200 copies a slab).  Hazards: the same accumulator comes round after 16 of these at least, the
-// fragments come from LDS; whoever reads acc afterwards calls settle() first.
+// them through both: 200 copies a slab).  The compiler puts no wait states around inline assembly, so they are part of it: two
+// in front of the instruction, for an operand or a scale that a vector instruction may have written last (issued while the
+// instruction before multiplies: no time); 32 behind the last one, in settle(), which hands the accumulators on.  What comes
+// between -- nothing but these instructions touches an accumulator -- the compiler decides: tests/test_f8_assembly.py looks at it.
 template <int TA, int TB>
 __device__ __forceinline__ void mma_pinned(const Frag<false> &b, const Frag<false> &a, f32x4 &acc) {
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
+  asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
                : "+a"(acc) : "v"(b.q), "v"(a.q), "v"(b.s), "v"(a.s), "n"(TB == BOF_E4M3 ? 0 : 1), "n"(TA == BOF_E4M3 ? 0 : 1));
 }
-__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+template <int X, int Y>
+__device__ __forceinline__ void settle(f32x4 (&acc)[X][Y]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < X * Y; x++) asm volatile("" : "+a"(acc[x / Y][x % Y]));
+}
 
 // A part of a product that is split along k writes its sums instead of C.
 __device__ __forceinline__ F8Product part_of(F8Product p, int z) {
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
     }
     __syncthreads();
   }
-  settle();
+  settle(acc);
   store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, max(tm * TM, i0 + wi), max(tn * TN, j0 + wj));
 }
 
@@ -608,7 +615,7 @@ __device__ __forceinline__ void ring_step(S &s, uint64_t a, uint64_t b, int sc, 
       asm volatile("" ::: "memory");
     }
     if (at == N) break;
-    mma_pinned<TA, TB>(fb[P][at / X], fa[P][at % X], acc[at % X][at / X]);
+    acc[at % X][at / X] = mma<TA, TB, false>(fb[P][at / X], fa[P][at % X], acc[at % X][at / X]);
     if (at < LAST) {
 #pragma unroll
       for (int w = at * WORK / LAST; w < (at + 1) * WORK / LAST; w++) {
@@ -752,10 +759,9 @@ __global__ void __launch_bounds__(256, X >= 4 && ST > 2 ? 1 : 2) f8_ring_kernel(
     __syncthreads();
     fragments(0);
 #pragma unroll
-    for (int at = 0; at < X * Y; at++) mma_pinned<TA, TB>(fb[0][at / X], fa[0][at % X], acc[at % X][at / X]);
+    for (int at = 0; at < X * Y; at++) acc[at % X][at / X] = mma<TA, TB, false>(fb[0][at / X], fa[0][at % X], acc[at % X][at / X]);
     __syncthreads();
   }
-  settle();
   store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, 0, 0);
 }
 
