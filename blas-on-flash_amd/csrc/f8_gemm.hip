@@ -279,6 +279,14 @@ __device__ __forceinline__ void touch(const uint8_t *from, uint32_t to) {
 }
 #pragma clang diagnostic pop
 
+// 16 bytes of memory (not of LDS or scratch, which the type says: a load through an address of any kind also counts as one of LDS,
+// and the wait for fragments in front of a barrier would wait for memory)
+__device__ __forceinline__ u32x4 load16(uint64_t from, uint32_t off) {
+  u32x4 v;
+  __builtin_memcpy(&v, (const uint8_t *) ((const __attribute__((address_space(1))) uint8_t *) from + off), 16);
+  return v;
+}
+
 // workgroups go round the 8 XCDs; tiles of one XCD are neighbours (each XCD has its own L2), GROUP rows of tiles deep
 __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int group, int &tm, int &tn) {
   const int nwg = tiles_m * tiles_n, q = nwg >> 3, r = nwg & 7, xcd = bid & 7, idx = bid >> 3;
@@ -371,7 +379,8 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
       dma16(b ? s.b_voff : s.a_voff, from, (b ? s.b_to + (P ^ 1) * S::B_IMAGE * 16 : s.a_to + P * S::A_IMAGE * 16) + r * 4096);
     } else {
       s.lds[s.put + (b ? S::B0 + (P ^ 1) * S::B_IMAGE : P * S::A_IMAGE) + r * 256] = s.staged[q];
-      __builtin_memcpy(&s.staged[q], reinterpret_cast<const uint8_t *>(from) + (b ? s.b_voff : s.a_voff), 16);
+      asm volatile("" ::: "memory");   // (the load into the same registers stays behind)
+      s.staged[q] = load16(from, b ? s.b_voff : s.a_voff);
     }
   };
   constexpr int N = X * Y, LAST = N - X;   // MFMAs, those in front of the barrier
@@ -465,9 +474,9 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
       dma16(s.a_voff, a_at(b0 + 1) + r * s.a_step, s.a_to + S::A_IMAGE * 16 + r * 4096);
     } else {
       u32x4 v[2];
-      __builtin_memcpy(&v[0], reinterpret_cast<const uint8_t *>(a_at(b0) + r * s.a_step) + s.a_voff, 16);
-      __builtin_memcpy(&v[1], reinterpret_cast<const uint8_t *>(a_at(b0 + 1) + r * s.a_step) + s.a_voff, 16);
-      __builtin_memcpy(&s.staged[Y + r], reinterpret_cast<const uint8_t *>(a_at(b0 + 2) + r * s.a_step) + s.a_voff, 16);
+      v[0] = load16(a_at(b0) + r * s.a_step, s.a_voff);
+      v[1] = load16(a_at(b0 + 1) + r * s.a_step, s.a_voff);
+      s.staged[Y + r] = load16(a_at(b0 + 2) + r * s.a_step, s.a_voff);
       lds[s.put + r * 256] = v[0];
       lds[s.put + S::A_IMAGE + r * 256] = v[1];
     }
@@ -478,8 +487,8 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
       dma16(s.b_voff, b_at(b0) + r * s.b_step, s.b_to + r * 4096);
     } else {
       u32x4 v;
-      __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(b_at(b0) + r * s.b_step) + s.b_voff, 16);
-      __builtin_memcpy(&s.staged[r], reinterpret_cast<const uint8_t *>(b_at(b0 + 1) + r * s.b_step) + s.b_voff, 16);
+      v = load16(b_at(b0) + r * s.b_step, s.b_voff);
+      s.staged[r] = load16(b_at(b0 + 1) + r * s.b_step, s.b_voff);
       lds[s.put + S::B0 + r * 256] = v;
     }
   }
@@ -593,7 +602,8 @@ __device__ __forceinline__ void ring_step(S &s, uint64_t a, uint64_t b, int sc, 
     } else {
       u32x4 &v = s.staged[P][q];
       s.lds[s.put + (AT + 3) % S::ST * S::BLOCK + q * 256] = v;
-      __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(from) + s.voff[q], 16);
+      asm volatile("" ::: "memory");   // (the load into the same registers stays behind)
+      v = load16(from, s.voff[q]);
     }
   };
   auto read = [&](int f) {   // fragment f of the next block
@@ -685,7 +695,7 @@ __global__ void __launch_bounds__(256, X >= 4 && ST > 2 ? 1 : 2) f8_ring_kernel(
         dma16(s.voff[r], from, s.to + u * S::BLOCK * 16 + r * 4096);
       } else {
         u32x4 v;
-        __builtin_memcpy(&v, reinterpret_cast<const uint8_t *>(from) + s.voff[r], 16);
+        v = load16(from, s.voff[r]);
         lds[s.put + u * S::BLOCK + r * 256] = v;
       }
     }
@@ -694,7 +704,7 @@ __global__ void __launch_bounds__(256, X >= 4 && ST > 2 ? 1 : 2) f8_ring_kernel(
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int r = 0; r < S::PIECES; r++)
-        __builtin_memcpy(&s.staged[u][r], reinterpret_cast<const uint8_t *>(r < S::PA ? a_at(b0 + 3 + u) : b_at(b0 + 3 + u)) + s.voff[r], 16);
+        s.staged[u][r] = load16(r < S::PA ? a_at(b0 + 3 + u) : b_at(b0 + 3 + u), s.voff[r]);
   }
   int seg = b0 >> 4;   // LDS has the scales of blocks 16 seg .. 16 seg + 31
   {
@@ -821,7 +831,7 @@ __global__ void __launch_bounds__(512, 1) f8_wide_kernel(F8Product q, int tiles_
       const uint64_t from = (a ? a_org + r * a_step : b_org + (r - X / 2) * b_step) + (uint64_t) min(blk, full - 1) * 128;
       const uint32_t off = CLAMP ? voff[CLAMP ? r : 0] : a ? a_voff : b_voff;
       if constexpr (DMA) dma16(off, from, to + slot * S::SLOT * 16 + r * 8192);
-      else __builtin_memcpy(&staged[r], reinterpret_cast<const uint8_t *>(from) + off, 16);
+      else staged[r] = load16(from, off);
     }
   };
   auto land = [&](int slot) {             // ... and there (staged)

@@ -146,6 +146,14 @@ def test_matrix_instructions_and_loads_to_lds_have_their_wait_states(kernels):
     assert not bad, "\n".join(f"{k}: {len(f)} places, the first: {f[0]}" for k, f in bad.items())
 
 
+def test_the_product_loads_memory_as_memory(kernels):
+    """A load through an address of any kind (flat) also counts as one of LDS: the wait for fragments in front of a barrier would
+    wait for the rows that are to arrive two steps later."""
+    for name, body in kernels.items():
+        if "f8_" in name:
+            assert not [i.op for i in body if i.op.startswith("flat_")], name
+
+
 MFMA = "v_mfma_scale_f32_16x16x128_f8f6f4 a[0:3], v[2:9], v[10:17], a[0:3], v18, v19 op_sel_hi:[0,0,0]"
 
 
