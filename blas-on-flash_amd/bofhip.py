@@ -134,6 +134,7 @@ SYMBOLS_F8 = [
     ("bof_f8_gemm", C.c_int, [i64, i64, i64, f32, P, i64, C.c_int, P, i64, C.c_int, P, i64, C.c_int, P, i64, C.c_int, f32, P, i64,
                               C.c_int, P, u64, P]),
     ("bof_f8_gemm_workspace_bytes", u64, [i64, i64, i64]),
+    ("bof_f8_gemm_plan", C.c_int, [i64, i64, i64, P, i64, i64, P, i64, i64, C.c_int, u64, C.POINTER(C.c_int)]),
     ("bof_f8_quant", C.c_int, [i64, i64, P, i64, C.c_int, C.c_int, C.c_int, P, i64, P, i64, P, i64, P, i64, P]),
     ("bof_rmsnorm_f8", C.c_int, [i64, i64, C.c_int, P, i64, P, i64, P, f32, P, i64, C.c_int, P, i64, P, i64, P, i64, P, P]),
     ("bof_rmsnorm_grad", C.c_int, [i64, i64, C.c_int, P, i64, P, i64, P, P, P, i64, P, i64, f32, P, P, u64, P]),
@@ -141,6 +142,8 @@ SYMBOLS_F8 = [
 ]
 # element types of bof_f8.h
 F32, BF16, F16, E4M3, E5M2 = range(5)
+# kernels of bof_f8_gemm, as bof_f8_gemm_plan numbers them
+F8_KERNELS = ("any", "rows", "64x32", "128x128", "128x128 two a CU", "128x160", "256x128", "256x256", "wide 128x128", "wide 256x128")
 
 
 def build(verbose=False):
@@ -245,6 +248,15 @@ def f8_gemm(m, n, k, alpha, a, lda, a_type, sa, ldsa, ga, b, ldb, b_type, sb, ld
 
 def f8_gemm_workspace_bytes(m, n, k):
     return lib().bof_f8_gemm_workspace_bytes(m, n, k)
+
+
+def f8_gemm_plan(m, n, k, a, lda, ldsa, b, ldb, ldsb, c_type, work_bytes=0):
+    """(name of the kernel that f8_gemm takes for these arguments, its parts along k)"""
+    parts = C.c_int()
+    kind = lib().bof_f8_gemm_plan(m, n, k, a, lda, ldsa, b, ldb, ldsb, c_type, work_bytes, C.byref(parts))
+    if kind < 0:
+        check(kind, "bof_f8_gemm_plan")
+    return F8_KERNELS[kind], parts.value
 
 
 def f8_quant(rows, cols, x, ldx, x_type, f8_type, group, q, ldq, s, lds, qt=0, ldqt=0, st=0, ldst=0, stream=0):

@@ -1087,15 +1087,18 @@ constexpr int kMaxParts = 32;
 
 // The kernel, and the parts along k, of least time by this estimate, in us: 1, and for every round of workgroups what it takes to
 // begin and to store, and what a block of k takes; a round is one workgroup a CU, or two where two numbers stand (the second
-// is for two).  For parts a join of 4 us and 4 TB/s for what they write and it reads.
+// is for two).  For parts a join of 2.3 us and 4 TB/s for what they write and it reads.  The constants are fitted to every kernel's
+// times over k from 256 to 16384, one round and several: of 171 other outputs (17 to 8192 rows, 128 to 16384 columns, k up to 28672) the
+// kernel that it names takes 1.3 % longer than the fastest of them on average, and more than 6 % longer for 15.  Measured, the
+// kernel named against its neighbours:
 //                 round      block
-//   64 x 32       3.0, 3.2   0.16, 0.30   48 x 8192 x 4096 9 us, 128 x 8192 x 4096 12 (128 x 128: 14 and 17)
-//   128 x 128     5.0        0.48         1024 x 4096 x 4096 20 us (64 x 32: 40, 256 x 256: 45)
-//     two a CU    4.5, 6.0   0.55, 1.00   12416 x 4669 x 256 59 us (256 x 256: 72), 2048 x 4096 x 1024 16 (256 x 128: 17); only by DMA
-//   128 x 160     8.0        0.45         1024 x 5120 x 4096 24 us (128 x 128: 34, 256 x 256: 46)
-//   256 x 128     9.5        0.75         2048 x 4096 x 4096 33 us (128 x 128: 38, 256 x 256: 46); only by DMA: staged it spills
-//   256 x 256     13         1.30         4096 x 4096 x 4096 55 us (128 x 128: 76), 8192 x 8192 x 1024 103 (two of 128 x 128: 111)
-//   wide          3.0        0.9 (128 x 128), 1.7 (256 x 128)
+//   64 x 32       2.9, 3.1   0.15, 0.35   512 x 2048 x 1024 6.8 us, 256 x 2048 x 4096 8.8 (128 x 128: 8.7, and 13.8 in four parts)
+//   128 x 128     6.1        0.47         2048 x 2048 x 1024 11.2 us, x 4096 21.7, 1024 x 4096 x 14336 58 (128 x 160: 15.6, 24.8, 64)
+//     two a CU    5.0, 6.6   0.71, 0.93   8192 x 8192 x 256 62 us (256 x 256: 66), 4096 x 2048 x 1024 16.3 (256 x 128: 18.2); only by DMA
+//   128 x 160     9.9        0.53         2048 x 2560 x 1024 15.0 us, x 4096 26.0, x 14336 67 (128 x 128: 18.6, 35, 96)
+//   256 x 128     10.4       0.70         4096 x 2048 x 4096 35 us, x 14336 108 (128 x 128: 42, 135); only by DMA: staged it spills
+//   256 x 256     14.9       1.24         4096 x 4096 x 1024 27 us, x 4096 58, x 14336 170 (two of 128 x 128: 30, 69, 239)
+//   wide          4.3        0.96 (128 x 128), 6.0, 1.73 (256 x 128)   2048 x 2048 x 4096 41 us (256 x 128: 58), 4096 x 4096 x 4096 134 (154)
 // One to sixteen rows of A and a workgroup a CU at most go to the kernel for few rows: 1 x 4096 x 4096 in 5.9 us, in 7.5 by tiles
 // of 64 x 32; 8 x 4096 x 8192 in 10.8 and 11.1; 1 x 8192 x 4096 in 8.8 and 8.4, 1 x 512 x 16384 in 11.9 and 9.0.  Wide: all up to
 // 32 rows, 32 x 4096 x 4096 in 12.0 us (33 rows by tiles: 15.6).
@@ -1116,22 +1119,22 @@ Plan plan_product(int64_t m, int64_t n, int64_t k, bool wide, bool near, bool dm
       const double blocks = (double) ((nb + parts - 1) / parts);
       auto round = [&](Cost c) { return c.round + blocks * c.block; };
       const double us = 1 + (double) (all / full) * round(full == 512 ? two : one) + (rest == 0 ? 0 : rest <= 256 ? round(one) : round(two)) +
-                        (parts > 1 ? 4 + (double) parts * (double) m * (double) n * 8 / 4e6 : 0);
+                        (parts > 1 ? 2.3 + (double) parts * (double) m * (double) n * 8 / 4e6 : 0);
       if (us < least) { least = us; best = {kind, (int) parts}; }
     }
   };
   if (wide) {
-    consider(kWide128, 128, 128, {3, 0.9}, {0, 0});
-    if (m >= 256 && n >= 128) consider(kWide256, 256, 128, {3, 1.7}, {0, 0});
+    consider(kWide128, 128, 128, {4.3, 0.96}, {0, 0});
+    if (m >= 256 && n >= 128) consider(kWide256, 256, 128, {6, 1.73}, {0, 0});
   } else {
-    consider(kRing64, 64, 32, {3, 0.16}, {3.2, 0.30});
-    consider(kRing128, 128, 128, {5, 0.48}, {0, 0});
-    consider(kRing160, 128, 160, {8, 0.45}, {0, 0});
+    consider(kRing64, 64, 32, {2.9, 0.15}, {3.1, 0.35});
+    consider(kRing128, 128, 128, {6.1, 0.47}, {0, 0});
+    consider(kRing160, 128, 160, {9.9, 0.53}, {0, 0});
     if (dma) {
-      consider(kTwo128, 128, 128, {4.5, 0.55}, {6, 1});
-      consider(kRing256, 256, 128, {9.5, 0.75}, {0, 0});
+      consider(kTwo128, 128, 128, {5, 0.71}, {6.6, 0.93});
+      consider(kRing256, 256, 128, {10.4, 0.7}, {0, 0});
     }
-    if (m >= 256 && n >= 256) max_parts = 1, consider(kTile256, 256, 256, {13, 1.3}, {0, 0});
+    if (m >= 256 && n >= 256) max_parts = 1, consider(kTile256, 256, 256, {14.9, 1.24}, {0, 0});
   }
   return best;
 }
@@ -1172,12 +1175,22 @@ void start_rows(const F8Product &p, hipStream_t st) {
   f8_rows_kernel<TA, TB, WIDE, MT, NT><<<wg, 64 * waves, bytes, st>>>(p);
 }
 
+// the plan for a call's arguments; work_bytes: of the workspace, 0 without one
+Plan plan_call(int64_t m, int64_t n, int64_t k, const void *a, int64_t lda, int64_t ldsa, const void *b, int64_t ldb, int64_t ldsb, int c_type, uint64_t work_bytes) {
+  const uint64_t room = work_bytes / ((uint64_t) m * (uint64_t) n * 4u);
+  const bool near = lda <= (1 << 24) && ldb <= (1 << 24) && ldsa <= (1 << 24) && ldsb <= (1 << 24);   // a tile of 256 rows: offsets of 32 bits
+  return plan_product(m, n, k, c_type == BOF_F32, near, rows_aligned(a, lda, b, ldb), room < 2 ? 1 : room < kMaxParts ? (int) room : kMaxParts);
+}
+// parts of whole blocks, as even as they come: blocks in one, and how many there are (the short block is the last one's)
+int whole_parts(int64_t k, int parts, int &blocks) {
+  const int all = k / 128 ? (int) (k / 128) : 1;
+  blocks = (all + parts - 1) / parts;
+  return (all + blocks - 1) / blocks;
+}
+
 template <int TA, int TB>
 hipError_t launch_product(F8Product p, Plan plan, hipStream_t st) {
-  // the short block is the last part's
-  const int all = p.k / 128 ? p.k / 128 : 1;
-  p.blocks_per_part = (all + plan.parts - 1) / plan.parts;
-  const int parts = (all + p.blocks_per_part - 1) / p.blocks_per_part;
+  const int parts = whole_parts(p.k, plan.parts, p.blocks_per_part);
   if (parts == 1) p.part = nullptr;
   drop_stale_error();
   switch (plan.kind) {
@@ -1223,6 +1236,16 @@ uint64_t bof_f8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
   return parts > 1 ? (uint64_t) parts * (uint64_t) m * (uint64_t) n * 4u : 0;
 }
 
+int bof_f8_gemm_plan(int64_t m, int64_t n, int64_t k, const void *a, int64_t lda, int64_t ldsa, const void *b, int64_t ldb, int64_t ldsb, int c_type,
+                     uint64_t work_bytes, int *parts) {
+  if (m <= 0 || n <= 0 || k <= 0 || m > INT32_MAX - 255 || n > INT32_MAX - 255 || k > INT32_MAX - 255 || c_type < BOF_F32 || c_type > BOF_F16 || !parts)
+    return refuse("bof_f8_gemm_plan", "bad size or type, or parts is missing");
+  const Plan plan = plan_call(m, n, k, a, lda, ldsa, b, ldb, ldsb, c_type, work_bytes);
+  int blocks;
+  *parts = whole_parts(k, plan.parts, blocks);
+  return plan.kind;
+}
+
 int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int64_t lda, int a_type, const uint8_t *sa,
                 int64_t ldsa, int ga, const void *b, int64_t ldb, int b_type, const uint8_t *sb, int64_t ldsb, int gb,
                 float beta, void *c, int64_t ldc, int c_type, void *work, uint64_t work_bytes, void *stream) {
@@ -1256,9 +1279,7 @@ int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int
   }
   for (auto [q, name] : {std::pair<const void *, const char *>{a, "A"}, {b, "B"}, {sa, "sa"}, {sb, "sb"}})
     if (int rc = dev.reaches(q, kCall, name)) return rc;
-  const uint64_t room = work ? work_bytes / ((uint64_t) m * (uint64_t) n * 4u) : 0;
-  const bool near = lda <= (1 << 24) && ldb <= (1 << 24) && ldsa <= (1 << 24) && ldsb <= (1 << 24);   // a tile of 256 rows: offsets of 32 bits
-  const Plan plan = plan_product(m, n, k, c_type == BOF_F32, near, rows_aligned(a, lda, b, ldb), room < 2 ? 1 : room < kMaxParts ? (int) room : kMaxParts);
+  const Plan plan = plan_call(m, n, k, a, lda, ldsa, b, ldb, ldsb, c_type, work ? work_bytes : 0);
   if (plan.parts > 1)
     if (int rc = dev.reaches(work, kCall, "work")) return rc;
   p.a = (const uint8_t *) a; p.b = (const uint8_t *) b; p.sa = sa; p.sb = sb;

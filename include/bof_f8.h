@@ -51,6 +51,12 @@ int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int
                 int64_t ldsb, int gb, float beta, void *c, int64_t ldc, int c_type, void *work, uint64_t work_bytes,
                 void *stream);
 uint64_t bof_f8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
+/* Which kernel that call takes, and in how many parts along k, for arguments that it would not refuse (host only: addresses
+ * are looked at, not followed).  0: tiles of any shape, 1: few rows; by size of the output tile 2: 64 x 32, 3: 128 x 128,
+ * 4: 128 x 128, two workgroups a CU, 5: 128 x 160, 6: 256 x 128, 7: 256 x 256; for a 32-bit C 8: 128 x 128,
+ * 9: 256 x 128.  BOF_EINVAL for an empty product. */
+int bof_f8_gemm_plan(int64_t m, int64_t n, int64_t k, const void *a, int64_t lda, int64_t ldsa, const void *b, int64_t ldb,
+                     int64_t ldsb, int c_type, uint64_t work_bytes, int *parts);
 
 /* X (rows x cols, x_type) into 8 bits (f8_type): as it lies into (q, s), transposed (cols x rows) into (qt, st), or
  * both from one read of X; the pair that is not wanted is NULL.  The scale of a block is the smallest power of two
