@@ -335,18 +335,6 @@ __device__ __forceinline__ void settle(f32x4 (&acc)[X][Y]) {
   for (int x = 0; x < X * Y; x++) asm volatile("" : "+a"(acc[x / Y][x % Y]));
 }
 
-// A part of a product that is split along k writes its sums instead of C.
-__device__ __forceinline__ F8Product part_of(F8Product p, int z) {
-  if (p.part) {
-    p.c = p.part + (int64_t) z * p.m * p.n;
-    p.c_type = BOF_F32;
-    p.ldc = p.n;
-    p.alpha = 1.f;
-    p.beta = 0.f;
-  }
-  return p;
-}
-
 template <int X, int Y, bool DMA>
 struct Slab {
   static constexpr int A_IMAGE = 256 * X, B_IMAGE = 256 * Y;       // chunks of 16 bytes in an image
@@ -421,10 +409,9 @@ __device__ __forceinline__ void slab(Slab<X, Y, DMA> &s, uint64_t b_next, uint64
 }
 
 template <int TA, int TB, int X, int Y, bool DMA>
-__global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product p, int tiles_m, int tiles_n) {
   using S = Slab<X, Y, DMA>;
   __shared__ u32x4 lds[S::CHUNKS];
-  const F8Product p = part_of(q, blockIdx.y);
   constexpr int TM = 32 * X, TN = 32 * Y;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
@@ -432,9 +419,7 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wi = (wave >> 1) * 16 * X, wj = (wave & 1) * 16 * Y;
   const int l16 = lane & 15, g = lane >> 4;
-  const int nb = (p.k + 127) >> 7, all = p.k >> 7;
-  const int b0 = blockIdx.y * p.blocks_per_part, full = min(all, b0 + p.blocks_per_part);   // slabs b0 .. full - 1, one at least
-  const bool tail = nb > all && blockIdx.y == gridDim.y - 1;
+  const int nb = (p.k + 127) >> 7, full = p.k >> 7;   // whole slabs, one at least
   S s;
   s.lds = lds;
   const int r8 = lane >> 3, chunk = (DMA ? (lane & 7) ^ r8 : lane & 7) << 4;
@@ -470,13 +455,13 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
 #pragma unroll
   for (int r = 0; r < X; r++) {
     if constexpr (DMA) {
-      dma16(s.a_voff, a_at(b0) + r * s.a_step, s.a_to + r * 4096);
-      dma16(s.a_voff, a_at(b0 + 1) + r * s.a_step, s.a_to + S::A_IMAGE * 16 + r * 4096);
+      dma16(s.a_voff, a_at(0) + r * s.a_step, s.a_to + r * 4096);
+      dma16(s.a_voff, a_at(1) + r * s.a_step, s.a_to + S::A_IMAGE * 16 + r * 4096);
     } else {
       u32x4 v[2];
-      v[0] = load16(a_at(b0) + r * s.a_step, s.a_voff);
-      v[1] = load16(a_at(b0 + 1) + r * s.a_step, s.a_voff);
-      s.staged[Y + r] = load16(a_at(b0 + 2) + r * s.a_step, s.a_voff);
+      v[0] = load16(a_at(0) + r * s.a_step, s.a_voff);
+      v[1] = load16(a_at(1) + r * s.a_step, s.a_voff);
+      s.staged[Y + r] = load16(a_at(2) + r * s.a_step, s.a_voff);
       lds[s.put + r * 256] = v[0];
       lds[s.put + S::A_IMAGE + r * 256] = v[1];
     }
@@ -484,21 +469,20 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
 #pragma unroll
   for (int r = 0; r < Y; r++) {
     if constexpr (DMA) {
-      dma16(s.b_voff, b_at(b0) + r * s.b_step, s.b_to + r * 4096);
+      dma16(s.b_voff, b_at(0) + r * s.b_step, s.b_to + r * 4096);
     } else {
       u32x4 v;
-      v = load16(b_at(b0) + r * s.b_step, s.b_voff);
-      s.staged[r] = load16(b_at(b0 + 1) + r * s.b_step, s.b_voff);
+      v = load16(b_at(0) + r * s.b_step, s.b_voff);
+      s.staged[r] = load16(b_at(1) + r * s.b_step, s.b_voff);
       lds[s.put + S::B0 + r * 256] = v;
     }
   }
-  const int seg = b0 >> 4;
   {
-    const u32x4 v[4] = {load_chunk(sa_row, seg * 16, nb), load_chunk(sb_row, seg * 16, nb), load_chunk(sa_row, seg * 16 + 16, nb), load_chunk(sb_row, seg * 16 + 16, nb)};
-    put_scales(half_of(seg), t, v[0]);
-    put_scales(half_of(seg), TM + t, v[1]);
-    put_scales(half_of(seg + 1), t, v[2]);
-    put_scales(half_of(seg + 1), TM + t, v[3]);
+    const u32x4 v[4] = {load_chunk(sa_row, 0, nb), load_chunk(sb_row, 0, nb), load_chunk(sa_row, 16, nb), load_chunk(sb_row, 16, nb)};
+    put_scales(half_of(0), t, v[0]);
+    put_scales(half_of(0), TM + t, v[1]);
+    put_scales(half_of(1), t, v[2]);
+    put_scales(half_of(1), TM + t, v[3]);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -506,14 +490,14 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
 #pragma unroll
   for (int x = 0; x < X; x++) {
     fa[0][x].q = both(lds[s.a_lo + x * 128], lds[s.a_hi + x * 128]);
-    fa[0][x].s = s.sa[byte_of(b0) + x * 320];
+    fa[0][x].s = s.sa[byte_of(0) + x * 320];
   }
   fb[0].q = both(lds[s.b_lo], lds[s.b_hi]);
-  fb[0].s = s.sb[byte_of(b0)];
+  fb[0].s = s.sb[byte_of(0)];
   __syncthreads();
-  int kb = b0;
+  int kb = 0;
   for (; kb + 2 <= full; kb += 2) {
-    if ((kb & 15) == 0 && kb > b0) {
+    if ((kb & 15) == 0 && kb > 0) {
       const u32x4 v[2] = {next_scales(sa_row, kb + 16, nb), next_scales(sb_row, kb + 16, nb)};
       put_scales(half_of((kb >> 4) + 1), t, v[0]);
       put_scales(half_of((kb >> 4) + 1), TM + t, v[1]);
@@ -524,13 +508,13 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
   if (kb < full) slab<TA, TB, X, Y, DMA, 0>(s, b_at(kb), a_at(kb), ahead_at(kb), byte_of(kb), byte_of(kb), fa, fb, acc);
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
-  if (tail) {   // the short block: through registers, zeros behind k
+  if (nb > full) {   // the short block: through registers, zeros behind k
     u32x4 v[X + Y];
 #pragma unroll
     for (int u = 0; u < X + Y; u++)
       v[u] = load_chunk_of_16(u < X ? p.a + (int64_t) (i0 + 32 * u + 8 * wave + r8) * p.lda : p.b + (int64_t) (j0 + 32 * (u - X) + 8 * wave + r8) * p.ldb,
-                        all * 128 + (lane & 7) * 16, p.k);
-    const uint8_t sa_last = sa_row[all], sb_last = sb_row[all];
+                        full * 128 + (lane & 7) * 16, p.k);
+    const uint8_t sa_last = sa_row[full], sb_last = sb_row[full];
 #pragma unroll
     for (int u = 0; u < X + Y; u++) lds[s.put + (u < X ? u * 256 : S::B0 + (u - X) * 256)] = v[u];
     scales[t * 20] = sa_last;
@@ -553,6 +537,18 @@ __global__ void __launch_bounds__(256, 1) f8_tile_kernel(F8Product q, int tiles_
   }
   settle(acc);
   store_wave<X, Y>(p, acc, (f32x4 *) lds + wave * (S::S0 / 4), i0 + wi, j0 + wj, max(tm * TM, i0 + wi), max(tn * TN, j0 + wj));
+}
+
+// A part of a product that is split along k writes its sums instead of C.
+__device__ __forceinline__ F8Product part_of(F8Product p, int z) {
+  if (p.part) {
+    p.c = p.part + (int64_t) z * p.m * p.n;
+    p.c_type = BOF_F32;
+    p.ldc = p.n;
+    p.alpha = 1.f;
+    p.beta = 0.f;
+  }
+  return p;
 }
 
 // ---- outputs of few tiles ------------------------------------------------------------

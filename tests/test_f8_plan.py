@@ -28,6 +28,14 @@ def test_long_sums_of_few_tiles_are_split():
     assert plan(512, 8192, 28672, work=0)[1] == 1
 
 
+def test_the_large_tiles_are_never_split():
+    """Their kernel has no parts."""
+    for m in (256, 300, 4096, 16384):
+        for n in (256, 1000, 8192):
+            for k in (128, 1000, 14336, 100000):
+                assert plan(m, n, k)[0] != "256x256" or plan(m, n, k)[1] == 1
+
+
 @pytest.mark.parametrize("wrong", [dict(m=0), dict(n=-1), dict(k=0), dict(k=2 ** 31), dict(c_type=bofhip.E4M3)])
 def test_empty_products_have_no_plan(wrong):
     with pytest.raises(bofhip.BofError, match="rc=-1"):
