@@ -1,7 +1,10 @@
 """CPU tests of bof_f8_gemm_plan (include/bof_f8.h): which kernel a product takes."""
+import itertools
+
 import pytest
 
 import bofhip
+import f8_shapes
 
 AT = 1 << 20   # an address, which nobody follows
 
@@ -34,6 +37,27 @@ def test_the_large_tiles_are_never_split():
         for n in (256, 1000, 8192):
             for k in (128, 1000, 14336, 100000):
                 assert plan(m, n, k)[0] != "256x256" or plan(m, n, k)[1] == 1
+
+
+@pytest.mark.parametrize("kernel,bits,aligned,m,n,k,parts,number", f8_shapes.each())
+def test_each_shape_takes_its_kernel(kernel, bits, aligned, m, n, k, parts, number):
+    c_type = bofhip.F32 if bits == 32 else bofhip.BF16
+    assert plan(m, n, k, c_type, f8_shapes.row_bytes(k, aligned), work=bofhip.f8_gemm_workspace_bytes(m, n, k)) == (kernel, parts)
+
+
+def test_the_shapes_go_every_way_through_every_kernel():
+    """(256 x 128 is split for long sums alone.)"""
+    assert {k for k, _, _ in f8_shapes.SHAPES} == set(bofhip.F8_KERNELS)
+    assert {k for k, _, aligned in f8_shapes.SHAPES if not aligned} == set(f8_shapes.STAGED)
+    for (kernel, _, _), shapes in f8_shapes.SHAPES.items():
+        ways = {f8_shapes.way(k, parts) for _, _, k, parts in shapes}
+        if kernel == "any":
+            assert all(k < 128 for _, _, k, _ in shapes) and len(shapes) == 4
+            continue
+        want = set(itertools.product([False, True] if kernel in f8_shapes.SPLIT else [False], [False, True], [False, True], [False, True]))
+        if kernel == "256x128":
+            want = {w for w in want if not w[0] or w[3]}
+        assert ways == want, kernel
 
 
 @pytest.mark.parametrize("wrong", [dict(m=0), dict(n=-1), dict(k=0), dict(k=2 ** 31), dict(c_type=bofhip.E4M3)])
