@@ -1245,6 +1245,7 @@ def headline_flash_gemm(bofhip, torch, dev, st, workdir, n, blk, io_threads, ste
         torch.cuda.synchronize()
         per, dumps = [], []
         L = bofhip.lib()
+        bounced = bofhip.file_bounced_bytes()
         t0 = time.perf_counter()
         for i in range(steps):
             per.append(step())
@@ -1253,6 +1254,7 @@ def headline_flash_gemm(bofhip, torch, dev, st, workdir, n, blk, io_threads, ste
                 L.bof_event_dump(dumps[-1].encode())
         torch.cuda.synchronize()
         dt = time.perf_counter() - t0
+        bounced = [(b - a) / max(steps, 1) for a, b in zip(bounced, bofhip.file_bounced_bytes())]
         launch_mix = bofhip.flash_last_launch_mix()
         ok = verify()
         if direct and probe:
@@ -1284,7 +1286,7 @@ def headline_flash_gemm(bofhip, torch, dev, st, workdir, n, blk, io_threads, ste
         del t
         torch.cuda.empty_cache()
     return {"dt": dt, "per_step": per, "warmup_steps": warm, "verified": bool(ok) and ok_warm is not False,
-            "verified_after_warmup": ok_warm, "odirect": direct, "create_files_s": round(create_s, 1),
+            "verified_after_warmup": ok_warm, "odirect": direct, "bounced_bytes_per_step": bounced, "create_files_s": round(create_s, 1),
             "file_system": _fs_of(workdir), "disk_probes": probes, "slowest_step_events": slow_events,
             "median_step_events": median_events, "launch_mix_last_step": launch_mix}
 
@@ -1421,7 +1423,10 @@ def run_single(args, bofhip, torch, dev, st):
         "config": {"workload": f"flash _gemm fp32 {n}x{n}x{n}, {blk}-tile, SSD-resident A/B/C, 1xMI355X",
                    "what_is_timed": "bof_flash_gemm on O_DIRECT files, page cache dropped, C write-back included "
                                     "(reference: drivers/gemm.cpp:57-62)",
-                   "odirect": h["odirect"], "file_system": h["file_system"], "io_threads": args.io_threads,
+                   "odirect": h["odirect"],
+                   # copied on their way, the kernel being unable to pin the staging buffers: read, written
+                   "odirect_GiB_copied_per_step": [round(b / 2**30, 3) for b in h["bounced_bytes_per_step"]],
+                   "file_system": h["file_system"], "io_threads": args.io_threads,
                    "compute_streams": args.streams or "library default (1)",
                    "tile_tasks_per_step": int(_mean(p["tasks"] for p in per)),
                    "GiB_read_per_step": round(mean_step["bytes_read"] / 2**30, 3),
@@ -1706,6 +1711,7 @@ def run_sharded(args, bofhip, torch, dev, st, rank, world, red_dev, one_gpu):
         if not good:
             break
     per_rank_s, agg_steps = [], []
+    bounced = bofhip.file_bounced_bytes()
     my_secs = []            # this rank's own seconds per timed step (gathered: `rank_mean_s` in the line)
     dt = float("nan")
     if good:
@@ -1733,9 +1739,10 @@ def run_sharded(args, bofhip, torch, dev, st, rank, world, red_dev, one_gpu):
     dist.all_reduce(rank_means)
     rank_means = [round(float(v), 3) for v in rank_means.tolist()]
     keys = ("bytes_read", "bytes_written", "bytes_peer", "bytes_h2d", "bytes_d2h", "kernel_launches", "kernel_seconds", "tasks")
-    agg = torch.tensor([sum(float(s.get(q, 0)) for s in agg_steps) for q in keys], dtype=torch.float64, device=red_dev)
+    bounced = [b - a for a, b in zip(bounced, bofhip.file_bounced_bytes())]
+    agg = torch.tensor([sum(float(s.get(q, 0)) for s in agg_steps) for q in keys] + [float(b) for b in bounced], dtype=torch.float64, device=red_dev)
     dist.all_reduce(agg)
-    agg = dict(zip(keys, [float(v) for v in agg.tolist()]))
+    agg = dict(zip((*keys, "bounced_read", "bounced_written"), [float(v) for v in agg.tolist()]))
     for fd in fds:
         bofhip.lib().bof_file_forget(fd)
         os.close(fd)
@@ -1795,6 +1802,8 @@ def run_sharded(args, bofhip, torch, dev, st, rank, world, red_dev, one_gpu):
                                     "B read from storage once per node, no data-path collective",
                    "parallelism": f"row-block x{world}", "ranks_seen": args.ranks_seen,
                    "backend": args.backend_seen, "odirect": was_direct,
+                   "odirect_GiB_copied_per_step": [round(agg[q] / args.steps / 2**30, 3)
+                                                   for q in ("bounced_read", "bounced_written")],
                    "file_dirs": (f"{D} directories ($BOF_BENCH_DIRS): per-rank A / C slab files, a replica of B in each"
                                  if local_slabs else "one shared A / B / C file set"),
                    "rank_s_min": round(min(a for a, _ in per_rank_s), 3), "rank_s_max": round(max(b for _, b in per_rank_s), 3),

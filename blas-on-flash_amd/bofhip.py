@@ -123,6 +123,7 @@ SYMBOLS = [
     ("bof_flash_last_launch_mix", C.c_int, [C.POINTER(C.c_uint64)]),
     ("bof_file_sread", C.c_int, [C.c_int, u64, u64, u64, u64, P, C.c_int]),
     ("bof_file_swrite", C.c_int, [C.c_int, u64, u64, u64, u64, P, C.c_int]),
+    ("bof_file_bounced_bytes", None, [C.POINTER(u64), C.POINTER(u64)]),
     ("bof_file_forget", C.c_int, [C.c_int]),
     ("bof_file_set_request_bytes", C.c_int, [u64]),
     ("bof_gen_dense", C.c_int, [P, i64, i64, chr_, u64, P]),
@@ -418,6 +419,14 @@ def flash_last_c_file():
     tw = C.c_uint64(0)
     mode = lib().bof_flash_last_c_file(C.byref(tw))
     return mode, tw.value
+
+
+def file_bounced_bytes():
+    """Bytes that O_DIRECT requests of this process read and wrote by way of the library's own memory, the kernel being
+    unable to pin their buffers."""
+    rd, wr = u64(), u64()
+    lib().bof_file_bounced_bytes(C.byref(rd), C.byref(wr))
+    return rd.value, wr.value
 
 
 def flash_last_device_stats():

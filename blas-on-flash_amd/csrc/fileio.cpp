@@ -96,6 +96,8 @@ void file_io_ops(uint64_t *reads, uint64_t *writes) {
   *reads = g_rd_ops.load();
   *writes = g_wr_ops.load();
 }
+// bytes of O_DIRECT requests that were copied through a Bounce
+static std::atomic<uint64_t> g_bounced_rd{0}, g_bounced_wr{0};
 
 // ---- per-thread AIO context -------------------------------------------------------
 struct AioCtx {
@@ -341,8 +343,10 @@ void unmap_for_forget(int fd) {
   std::unique_lock<std::mutex> lk(g_map_mu);
   unmap_locked(fd, lk);
 }
+static void drop_idle_bounces();
 // every write mapping goes (bof_flash_release), each once its stores in flight are done
 void file_unmap_all() {
+  drop_idle_bounces();
   std::unique_lock<std::mutex> lk(g_map_mu);
   while (!g_map.empty()) unmap_locked(g_map.begin()->first, lk);
 }
@@ -365,11 +369,103 @@ static int rw_full(int fd, bool wr, char *buf, uint64_t len, uint64_t off) {
   return 0;
 }
 
+static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_t n_strides, uint64_t len, void *buf, bool use_aio,
+                      bool may_bounce = true);
+
 // A buffer the kernel cannot pin -- the pinned memory of some machines is a mapping of the GPU driver's without pages of its
-// own -- makes every O_DIRECT request of it end in EFAULT: such a request goes through the buffered twin, which copies (and
-// still reports EFAULT for an address that is none).
+// own -- makes every O_DIRECT request of it end in EFAULT.  Such a request is made of memory that can be pinned, a piece at a time,
+// and copied: it stays O_DIRECT, at the device's rate and without pages in the page cache.  The memory is a mapping of a file in
+// memory, and the copies are reads and writes of that file: the kernel makes them, so that an address that is none still ends
+// in EFAULT.  One a thread, leased like its AIO context; idle ones go with the mappings (file_unmap_all).
+namespace {
+struct Bounce {
+  uint64_t size;   // $BOF_BOUNCE_KIB, 16 MiB: four requests of the default size in flight
+  int fd = -1;
+  char *at = nullptr;
+  Bounce() {
+    const char *e = getenv("BOF_BOUNCE_KIB");
+    size = (uint64_t) std::min(std::max(e ? atol(e) : 16384l, 64l), 1l << 20) / 64 << 16;   // (multiples of the largest O_DIRECT alignment)
+    fd = (int) syscall(SYS_memfd_create, "bof bounce", 1u /* MFD_CLOEXEC */);
+    if (fd < 0 || ::ftruncate(fd, (off_t) size) != 0) return;
+    void *p = ::mmap(nullptr, size, PROT_READ | PROT_WRITE, MAP_SHARED, fd, 0);
+    if (p != MAP_FAILED) at = (char *) p;
+  }
+  ~Bounce() {
+    if (at) ::munmap(at, size);
+    if (fd >= 0) ::close(fd);
+  }
+  Bounce(const Bounce &) = delete;
+  Bounce &operator=(const Bounce &) = delete;
+  // n bytes from its beginning to `to`, or from `from` to its beginning
+  int copy_out(char *to, uint64_t n) { return copy(n, [&](uint64_t done) { return ::pread(fd, to + done, n - done, (off_t) done); }); }
+  int copy_in(const char *from, uint64_t n) { return copy(n, [&](uint64_t done) { return ::pwrite(fd, from + done, n - done, (off_t) done); }); }
+
+ private:
+  template <class F>
+  static int copy(uint64_t n, F &&some) {
+    for (uint64_t done = 0; done < n;) {
+      const ssize_t r = some(done);
+      if (r < 0 && errno == EINTR) continue;
+      if (r <= 0) return r < 0 ? -errno : -EIO;
+      done += (uint64_t) r;
+    }
+    return 0;
+  }
+};
+struct BouncePool {
+  std::mutex mu;
+  std::vector<Bounce *> idle;
+  Bounce *get() {
+    {
+      std::lock_guard<std::mutex> lk(mu);
+      if (!idle.empty()) { Bounce *b = idle.back(); idle.pop_back(); return b; }
+    }
+    return new Bounce();
+  }
+  void put(Bounce *b) {
+    if (!b->at) { delete b; return; }
+    std::lock_guard<std::mutex> lk(mu);
+    idle.push_back(b);
+  }
+  void clear() {
+    std::lock_guard<std::mutex> lk(mu);
+    for (Bounce *b : idle) delete b;
+    idle.clear();
+  }
+  ~BouncePool() { clear(); }
+};
+BouncePool &bounce_pool() {
+  static BouncePool p;
+  return p;
+}
+}  // namespace
+
+static void drop_idle_bounces() { bounce_pool().clear(); }
+
+static int bounced_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_t n_strides, uint64_t len, char *p, bool use_aio) {
+  struct Lease {
+    Bounce *b = bounce_pool().get();
+    ~Lease() { bounce_pool().put(b); }
+  } lease;
+  Bounce &b = *lease.b;
+  if (!b.at) return -EFAULT;
+  // pieces of a stride, or several strides
+  const uint64_t part = std::min(len, b.size), many = len < b.size ? b.size / len : 1;
+  for (uint64_t s = 0; s < n_strides; s += many)
+    for (uint64_t o = 0; o < len; o += part) {
+      const uint64_t n = std::min(many, n_strides - s), size = std::min(part, len - o), from = offset + s * stride + o;
+      char *const user = p + s * len + o;
+      int rc = wr ? b.copy_in(user, n * size) : 0;
+      if (!rc) rc = strided_io(fd, wr, from, stride, n, size, b.at, use_aio, false);
+      if (!rc && !wr) rc = b.copy_out(user, n * size);
+      if (rc) return rc;
+      (wr ? g_bounced_wr : g_bounced_rd) += n * size;
+    }
+  return 0;
+}
+
 static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_t n_strides,
-                      uint64_t len, void *buf, bool use_aio) {
+                      uint64_t len, void *buf, bool use_aio, bool may_bounce) {
   if (n_strides == 0 || len == 0) return 0;
   if (n_strides > 1 && stride == len) {  // dense region: one contiguous transfer
     len *= n_strides;
@@ -393,7 +489,8 @@ static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_
       for (uint64_t o = 0; o < len; o += piece)
         pieces.push_back(IoPiece{fd, wr, p + s * len + o, std::min(piece, len - o), offset + s * stride + o});
     const int rc = uring_run(pieces);
-    if (rc != -ENOSYS && rc != -EFAULT) {
+    if (rc == -EFAULT && may_bounce) return bounced_io(fd, wr, offset, stride, n_strides, len, p, use_aio);
+    if (rc != -ENOSYS) {
       (wr ? g_wr_ops : g_rd_ops) += pieces.size();
       return rc;
     }
@@ -415,17 +512,16 @@ static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_
       }
     }
     const int rc = aio_run(cbs);
-    if (rc != -ENOSYS && rc != -EFAULT) {
+    if (rc == -EFAULT && may_bounce) return bounced_io(fd, wr, offset, stride, n_strides, len, p, use_aio);
+    if (rc != -ENOSYS) {
       (wr ? g_wr_ops : g_rd_ops) += cbs.size();
       return rc;
     }
   }
   for (uint64_t s = 0; s < n_strides; s++) {
-    int rc = rw_full(fd, wr, p + s * len, len, offset + s * stride);
-    if (rc == -EFAULT && direct && aligned) {
-      const int twin = buffered_twin(fd);
-      rc = twin < 0 ? -EBADF : rw_full(twin, wr, p + s * len, len, offset + s * stride);
-    }
+    const int rc = rw_full(fd, wr, p + s * len, len, offset + s * stride);
+    if (rc == -EFAULT && direct && aligned && may_bounce)
+      return bounced_io(fd, wr, offset + s * stride, stride, n_strides - s, len, p + s * len, use_aio);
     if (rc) return rc;
   }
   return 0;
@@ -508,6 +604,10 @@ extern "C" int bof_file_set_request_bytes(uint64_t bytes) {
   if (bytes < 512 || bytes % 512) { bof::set_error("bof_file_set_request_bytes: need a multiple of 512"); return BOF_EINVAL; }
   bof::g_req_bytes.store(std::min<uint64_t>(bytes, bof::kMaxChunk));
   return BOF_OK;
+}
+extern "C" void bof_file_bounced_bytes(uint64_t *read, uint64_t *written) {
+  if (read) *read = bof::g_bounced_rd.load();
+  if (written) *written = bof::g_bounced_wr.load();
 }
 extern "C" int bof_file_forget(int fd) {
   bof::file_forget(fd);

@@ -457,6 +457,10 @@ int bof_file_swrite(int fd, uint64_t offset, uint64_t stride, uint64_t n_strides
  * default 4 MiB or $BOF_IO_REQUEST_KIB.  Multiple of 512, at most 32 MiB (the reference's
  * MAX_CHUNK_SIZE, flash_file_handle.cpp:25). */
 int bof_file_set_request_bytes(uint64_t bytes);
+/* Bytes of O_DIRECT requests that this process has read and written by way of memory of the library's own, because the
+ * kernel cannot pin the caller's (on some machines hipHostMalloc's memory is a mapping without pages of its own, and
+ * O_DIRECT requests of it end in EFAULT).  They stay O_DIRECT and cost a copy.  Either may be NULL. */
+void bof_file_bounced_bytes(uint64_t *read, uint64_t *written);
 /* Unaligned requests on an O_DIRECT descriptor go through a cached buffered descriptor of
  * the same file, and large buffered writes into cached pages through a shared mapping of it
  * (BOF_MMAP_WRITES=0 turns the mapping off).  Both are keyed by the descriptor NUMBER: calling
