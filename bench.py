@@ -35,6 +35,11 @@ MFMA_F32_PEAK_TFLOPS = 157.3   # MI355X_MICROARCH.md: 256 CU x 2.4 GHz x 256 flo
 HBM_PEAK_GBS = 8000.0
 
 
+def _progress(what):
+    """A line on stderr after each part of a run that takes minutes (stdout carries the result line alone)."""
+    print(f"bench.py: {what}", file=sys.stderr, flush=True)
+
+
 def _best_of(fn, reps):
     best = float("inf")
     for _ in range(reps):
@@ -1054,6 +1059,7 @@ def e2e_block(bofhip, torch, dev, st, args, gemm_kernel_s, csrmm_kernel_s, gemm6
             # (the O_DIRECT form of this configuration is the headline itself)
             out["gemm"] = e2e_gemm(bofhip, torch, dev, st, workdir, n, args.blk, gemm_kernel_s, args.io_threads,
                                    args.e2e_reps, modes=("buffered",))
+            _progress("gemm from files")
         else:
             out["gemm"] = {"skipped": "not enough free disk for three matrix files"}
         bofhip.lib().bof_flash_release()
@@ -1065,6 +1071,7 @@ def e2e_block(bofhip, torch, dev, st, args, gemm_kernel_s, csrmm_kernel_s, gemm6
                 # (two calls: the first pays the cold allocations of 48 GiB of panel slots, the second is the steady state)
                 out["gemm_65536"] = e2e_gemm(bofhip, torch, dev, st, workdir, 65536, args.blk, gemm64_kernel_s,
                                              args.io_threads, 2, modes=("odirect",))
+                _progress("gemm_65536 from files")
             else:
                 out["gemm_65536"] = {"skipped": f"needs 48 GiB of scratch disk, {free / 2**30:.0f} GiB free"}
             bofhip.lib().bof_flash_release()
@@ -1093,12 +1100,14 @@ def e2e_block(bofhip, torch, dev, st, args, gemm_kernel_s, csrmm_kernel_s, gemm6
             pass
         elif free > 19e9:
             out["csrmm"] = e2e_csrmm(bofhip, torch, dev, st, workdir, csrmm_kernel_s, args.io_threads, args.e2e_reps)
+            _progress("csrmm from files")
         else:
             out["csrmm"] = {"skipped": "not enough free disk for the cfg3 files (17.7 GB)"}
         bofhip.lib().bof_flash_release()
         if not (args.no_csr or args.e2e_size != 32768):
             if shutil.disk_usage(workdir).free > 8e9:
                 out["csrgemv"] = e2e_csrgemv(bofhip, torch, dev, st, workdir, gemv_kernel_ms, args.io_threads, args.e2e_reps)
+                _progress("csrgemv from files")
             else:
                 out["csrgemv"] = {"skipped": "not enough free disk for the cfg5-size files (6.4 GB)"}
             bofhip.lib().bof_flash_release()
@@ -1186,6 +1195,7 @@ def headline_flash_gemm(bofhip, torch, dev, st, workdir, n, blk, io_threads, ste
     t.zero_()
     _write_device_tensor(bofhip, t, pc, True, wopts, st)                    # dense_create mode z
     create_s = time.perf_counter() - t0
+    _progress(f"three files of {nbytes / 2**30:.0f} GiB in {create_s:.1f} s")
     rowpat = _closed_form_rows(torch, dev, n, n, n)
     idx = torch.arange(n, device=dev)
 
@@ -1240,6 +1250,7 @@ def headline_flash_gemm(bofhip, torch, dev, st, workdir, n, blk, io_threads, ste
                 return {"when": label, "error": f"{type(e).__name__}: {e}"[:200]}
         if direct and probe:
             probes.append(safe_probe("before the timed steps"))
+        _progress(f"{warmup} warm-up steps")
         reset_c()                                   # the timed steps must produce C, not find it
         _drop_cache((pa, pb, pc))
         torch.cuda.synchronize()
@@ -1255,6 +1266,7 @@ def headline_flash_gemm(bofhip, torch, dev, st, workdir, n, blk, io_threads, ste
         torch.cuda.synchronize()
         dt = time.perf_counter() - t0
         bounced = [(b - a) / max(steps, 1) for a, b in zip(bounced, bofhip.file_bounced_bytes())]
+        _progress(f"{steps} steps in {dt:.1f} s")
         launch_mix = bofhip.flash_last_launch_mix()
         ok = verify()
         if direct and probe:
@@ -1360,6 +1372,7 @@ def run_single(args, bofhip, torch, dev, st):
         except Exception as e:
             ceil = {"error": f"{type(e).__name__}: {str(e)[:200]}"}
         detail["ceilings"] = ceil
+        _progress("disk and PCIe rates")
         bofhip.lib().bof_flash_release()
         evdir = os.path.join(workdir, "events")
         os.makedirs(evdir, exist_ok=True)
@@ -1464,6 +1477,7 @@ def run_single(args, bofhip, torch, dev, st):
     if not args.no_cpu:
         cb = cpu_baseline(with_csr=not args.no_extras and not args.size, full_step=not args.size and not args.no_cpu_full_step)
         detail["cpu_baseline"] = cb
+        _progress("CPU baseline")
         line["cpu_baseline"] = {"value": cb.get("value"), "unit": cb.get("unit", "GFLOP/s"), "cores": cb.get("cores"),
                                 "kind": cb.get("kind", "port"),
                                 "sample": "in-memory MKL, sampled (not the reference's flash path on files): "
@@ -1493,6 +1507,7 @@ def extras_single(args, bofhip, torch, dev, st, detail, gemm_kernel_s):
         r = resident_gemm_line(bofhip, torch, dev, st, 32768, 32768, 32768, 0, args.blk, 1, 3,
                                "cfg2 tile DAG, A/B/C resident in HBM (I/O skipped)")
         detail["resident_cfg2"] = r
+        _progress("resident product")
         ex["resident_cfg2_gflops"] = r["gflops"]
         ex["resident_cfg2_frac_mfma"] = r["frac_of_mfma_peak"]
         ex["resident_rel_err_vs_f64"] = float(f"{r['first_tile_row_rel_err_vs_float64']:.2e}")
@@ -1509,6 +1524,7 @@ def extras_single(args, bofhip, torch, dev, st, detail, gemm_kernel_s):
         except Exception as e:
             sec["kmeans_error"] = str(e)[:200]
         detail["secondary"] = sec
+        _progress("resident CSR products and kmeans")
         if isinstance(sec.get("csrmm"), dict):
             r3 = sec["csrmm"]["roofline"]
             ex["csrmm_kernel_ms"] = sec["csrmm"]["ms"]
