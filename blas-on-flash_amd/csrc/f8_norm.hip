@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_grad_kernel(Norm
           const float g = dy[i].at(e), xhat = h[i].at(e) * rstd;
           v[e] = rstd * (g * w[i].at(e) - xhat * mean);
           if (p.dh) v[e] += dh[i].at(e);
-          if (KEEP) dw[i][e] += g * xhat;
+          if (KEEP) dw[i][e] = fmaf(g, xhat, dw[i][e]);
         }
         store_eight<T>(p.dx, row * p.lddx + c, v, valid);
         if (!KEEP && part) {
@@ -318,8 +318,8 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) norm_grad_kernel(Norm
 #pragma unroll
           for (int e = 0; e < 8; e++)
             if (e < valid) {
-              const float g = dy[i].at(e) * (h[i].at(e) * rstd);
-              part[c + e] = first ? g : part[c + e] + g;
+              const float xhat = h[i].at(e) * rstd;
+              part[c + e] = first ? dy[i].at(e) * xhat : fmaf(dy[i].at(e), xhat, part[c + e]);
             }
         }
       }

@@ -81,7 +81,7 @@ int bof_rmsnorm_f8(int64_t rows, int64_t n, int type, const void *x, int64_t ldx
  *     g = dy * w,   xhat = h * rstd,   dx = rstd * (g - xhat * mean(g * xhat)) + dh,   dw = beta * dw + sum over rows of dy * xhat
  * dx (of `type`) is the gradient of X and of R; it may be dy or dh itself.  dw: n floats, or NULL; beta == 0: not read.
  * dw needs `work` of bof_rmsnorm_grad_workspace_bytes(rows, n) bytes (16-byte aligned); rows are summed in a fixed
- * order. */
+ * order, their products unrounded (fused). */
 int bof_rmsnorm_grad(int64_t rows, int64_t n, int type, const void *dy, int64_t lddy, const void *h, int64_t ldh,
                      const void *w, const float *rstd, const void *dh, int64_t lddh, void *dx, int64_t lddx, float beta,
                      float *dw, void *work, uint64_t work_bytes, void *stream);
