@@ -376,10 +376,12 @@ static int strided_io(int fd, bool wr, uint64_t offset, uint64_t stride, uint64_
 // own -- makes every O_DIRECT request of it end in EFAULT.  Such a request is made of memory that can be pinned, a piece at a time,
 // and copied: it stays O_DIRECT, at the device's rate and without pages in the page cache.  The memory is a mapping of a file in
 // memory, and the copies are reads and writes of that file: the kernel makes them, so that an address that is none still ends
-// in EFAULT.  One a thread, leased like its AIO context; idle ones go with the mappings (file_unmap_all).
+// in EFAULT.  One a thread, leased like its AIO context; idle ones go with the mappings (file_unmap_all), and a process that was
+// forked makes its own: its parent's are the same pages.
 namespace {
 struct Bounce {
   uint64_t size;   // $BOF_BOUNCE_KIB, 16 MiB: four requests of the default size in flight
+  const pid_t owner = ::getpid();
   int fd = -1;
   char *at = nullptr;
   Bounce() {
@@ -416,9 +418,13 @@ struct BouncePool {
   std::mutex mu;
   std::vector<Bounce *> idle;
   Bounce *get() {
-    {
-      std::lock_guard<std::mutex> lk(mu);
-      if (!idle.empty()) { Bounce *b = idle.back(); idle.pop_back(); return b; }
+    const pid_t me = ::getpid();
+    std::lock_guard<std::mutex> lk(mu);
+    while (!idle.empty()) {
+      Bounce *b = idle.back();
+      idle.pop_back();
+      if (b->owner == me) return b;
+      delete b;
     }
     return new Bounce();
   }

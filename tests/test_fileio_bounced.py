@@ -122,6 +122,47 @@ def test_they_arrive_whole_in_pieces(tmp_path, engine, stride, n, length):
     assert r.returncode == 0 and "whole" in r.stdout, (r.returncode, r.stdout, r.stderr)
 
 
+FORKED = """
+import ctypes, mmap, os, sys
+import numpy as np
+import bofhip
+L, path, size = bofhip.lib(), sys.argv[1], 1 << 20
+secret = ctypes.CDLL(None, use_errno=True).syscall(447, 0)     # memfd_secret
+if secret < 0:
+    sys.exit(print("skip: no memfd_secret"))
+os.ftruncate(secret, 2 * size)
+try:
+    buf = np.frombuffer(mmap.mmap(secret, 2 * size), np.uint8)
+    buf[:] = 0
+except OSError:
+    sys.exit(print("skip: no room for secret memory"))
+data = np.random.default_rng(2).integers(0, 256, 2 * size, np.uint8)
+data.tofile(path)
+fd = os.open(path, os.O_RDWR | os.O_DIRECT)
+def read(part):
+    mine = buf[part * size:(part + 1) * size]
+    mine[:] = 0
+    assert L.bof_file_sread(fd, part * size, 0, 1, size, mine.ctypes.data, 0) == 0, L.bof_last_error()
+    return np.array_equal(mine, data[part * size:(part + 1) * size])
+assert read(0) and bofhip.file_bounced_bytes()[0] == size
+child = os.fork()
+good = all([read(child == 0) for _ in range(200)])
+if child == 0:
+    os._exit(0 if good else 1)
+assert os.waitstatus_to_exitcode(os.waitpid(child, 0)[1]) == 0 and good
+print("apart")
+"""
+
+
+def test_a_forked_process_has_its_own(tmp_path):
+    """Parent and child read at once what each of them has to copy: neither finds the other's bytes."""
+    r = subprocess.run([sys.executable, "-c", FORKED, str(tmp_path / "data")], cwd=HERE, capture_output=True, text=True, timeout=120,
+                       env=dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path)))
+    if "skip" in r.stdout:
+        pytest.skip(r.stdout)
+    assert r.returncode == 0 and "apart" in r.stdout, (r.returncode, r.stdout, r.stderr)
+
+
 BAD_WRITE = """
 import os, sys
 import bofhip
