@@ -45,7 +45,9 @@ extern "C" {
  * 2^-10 of the sum of those largest products; for a 32-bit C the operands are widened exactly and nothing is cut
  * (elements whose value leaves the range of bf16 become 0 or infinite, as in fp32).
  * work: optional.  With bof_f8_gemm_workspace_bytes(m, n, k) bytes (16-byte aligned) a product with few output tiles
- * is split along k and its parts are added in a fixed order; with less or NULL it is split less or not at all. */
+ * is split along k and its parts are added in a fixed order; with less or NULL it is split less or not at all.  The order of
+ * the sums, and with it their last bits, is that of the kernel and the parts which bof_f8_gemm_plan names: the same
+ * sizes, alignment and work_bytes give the same bits. */
 int bof_f8_gemm(int64_t m, int64_t n, int64_t k, float alpha, const void *a, int64_t lda, int a_type,
                 const uint8_t *sa, int64_t ldsa, int ga, const void *b, int64_t ldb, int b_type, const uint8_t *sb,
                 int64_t ldsb, int gb, float beta, void *c, int64_t ldc, int c_type, void *work, uint64_t work_bytes,
